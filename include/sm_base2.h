@@ -249,6 +249,67 @@ int sm_plate_product_rows_noalloc(const sm_plate* p, const int64_t* x16, int32_t
 /* bytes of the device plate (for bandwidth accounting) */
 int64_t sm_plate_bytes(const sm_plate* p);
 
+/* ---------------------------------------------------------------------------------------------------
+ * Operators in few bits, on caller-owned DEVICE buffers: plates of 8-bit digits, and a cache of 4 or 8-bit digits with the
+ * attention that reads it.  No counterpart in the reference, whose plates and lights have 16 bits; the arithmetic is its
+ * own (base2.py:18-53, 85-100) on fewer.  With rsh(x, s) = x 2^-s rounded half up, a row's digits of b bits are
+ *     sh = max(bitlen(OR |x|) - (b - 1), 0),   digit = clamp(rsh(x, sh), -2^(b-1), 2^(b-1) - 1)   worth digit 2^sh.
+ * Calls only launch kernels on their stream: none allocates, waits or keeps anything, so all may be captured into a graph,
+ * and calls may overlap where their outputs, caches and workspaces are their own.  A call runs on the device that holds
+ * the plate or the cache, whatever device is current; its stream has to be one of that device.
+ * ------------------------------------------------------------------------------------------------- */
+#define SM_PLATE8_NIN 131071      /* a pile of 8-bit digits stays within int32 */
+#define SM_PLATE8_ROWS (1 << 20)
+typedef struct sm_plate8 sm_plate8;
+/* from an input-major int8 [nin][nout] host array, each column's power of two (within +-1024) and bias at the stream's
+ * 2^-16 (convert.py: cols8, stream); any nin up to SM_PLATE8_NIN and nout up to 2^24 */
+int sm_plate8_create(const int8_t* w, const int32_t* e, const int64_t* b, int32_t nin, int32_t nout, sm_plate8** out);
+int sm_plate8_destroy(sm_plate8* p);
+int64_t sm_plate8_bytes(const sm_plate8* p);                     /* of the device plate (for bandwidth accounting) */
+int64_t sm_plate8_work(const sm_plate8* p, int32_t rows);        /* bytes of workspace of a product of `rows` rows */
+/* out[r][j] = rsh(sum_i x8[r][i] w[i][j], -(e[j] + ex[r] + 16)) + b[j] for r < rows, with row r's 8-bit digits x8 and their
+ * level ex = sh - 16: a scale for each token and each channel.  X: device int64 rows at 2^-16, x_stride values apart; out:
+ * device int64 rows, out_stride apart.  work: sm_plate8_work bytes of device memory at 16 bytes' alignment, used until the
+ * call's kernels have run.  rows 0 .. SM_PLATE8_ROWS. */
+int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x_stride, int32_t rows, int64_t* out, int64_t out_stride,
+                      void* work, int64_t work_bytes, void* stream);
+
+/* The shape of a cache: keys and values of `streams` streams, ctx positions, `heads` key heads of dim dimensions, digits of
+ * `bits` bits (4 or 8) and one level (sh, a byte) for each (stream, position, head) row of k and of v.  The cache is
+ * sm_narrow_bytes bytes of device memory at 16 bytes' alignment; zeroed memory is an empty cache.  Its layout is at the
+ * head of the cache's kernels (csrc/sm_narrow.hip): tiles of 64 positions, each (stream, head)'s in a row. */
+typedef struct { int32_t streams, heads, dim, ctx, bits; } sm_narrow;
+int64_t sm_narrow_bytes(const sm_narrow* c);                     /* negative on error */
+/* Rows of k and v (device int64 at 2^-16) into the cache: row t < count[s] of stream s goes to position start[s] + t of all
+ * its heads.  Row t of stream s is at k + s stream_stride + t row_stride, its heads' dim values each in a row (strides in
+ * values, so k and v may be parts of one wider row).  start and count: device int32 [streams]; count NULL: `rows` for
+ * every stream.  Rows past count[s] and positions outside 0 .. ctx - 1 are left out.  Calls that write the same (stream,
+ * head)'s tile of 64 positions have to be in order. */
+int sm_narrow_write(const sm_narrow* c, void* cache, const int64_t* k, const int64_t* v, int64_t row_stride,
+                    int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream);
+/* The same rows back: what the digits stand for, digit 2^sh.  Rows that are left out stay as they are in k and v. */
+int sm_narrow_read(const sm_narrow* c, const void* cache, int64_t* k, int64_t* v, int64_t row_stride,
+                   int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream);
+/* Attention of `rows` rows a stream over the cache: row t < count[s] of stream s is at position p = start[s] + t, and each of
+ * its q_heads query heads (a multiple of heads; head i reads key head i / (q_heads / heads)) sees positions 0 .. p, which
+ * hold that row's own k and v already.  span: no row's position reaches it (at most ctx; the call's cost follows it).  Rows
+ * past count[s] and rows whose position is not in 0 .. span - 1 are left out: their out stays as it is.
+ * scale: log2 of the scores' scale at 2^-16 (-(log2(dim) / 2) 65536 for the usual 1 / sqrt(dim)), within +-2^22.
+ * For one row (ARR, EXP2, log2fix and power are the tables' and base2.py:42-53):
+ *     q16, eq = to16(q);  q8, sh the 8-bit digits of q16 EXP2[scale & 0xFFFF];  eq += (scale >> 16) - 16 + sh
+ *     score of position i   sc = clamp(rsh(sum_d q8_d k_id, -(eq + level_i - 16 + 10)), -2^30, 2^30)
+ *     chunk of 256 positions, of those seen   m = max sc, E = max value level, u_i = rsh(ARR[m - sc_i], 2),
+ *         A = sum u_i, N = rsh(sum_i rsh(u_i, E - level_i) v_i, 8)
+ *     the row, with its chunks' largest m and E as M and L and f = ARR[M - m]
+ *         out = power(sum rsh(N f, 24 + L - E), (L + 8) 65536 - log2fix(sum rsh(A f, 24)))
+ * Every sum is exact, so no launch shape changes a result.  q, out: device int64, strides in values as for k.
+ * work: sm_narrow_work bytes of device memory at 16 bytes' alignment, used until the call's kernels have run. */
+int64_t sm_narrow_work(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span);   /* negative on error */
+int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const void* cache, const int64_t* q, int64_t q_row,
+                     int64_t q_stream, int32_t q_heads, int32_t rows, int32_t span, const int32_t* start,
+                     const int32_t* count, int32_t scale, int64_t* out, int64_t out_row, int64_t out_stream, void* work,
+                     int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

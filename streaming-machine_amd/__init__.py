@@ -8,7 +8,7 @@ Host API, after the reference's "convert -> layout -> stream" (base2_convert.py,
     ids  = m.stream(prompt_ids, n_words)        # greedy words, decoded on the GPU
     word = m.forward(ids)                       # base2.py:forward's contract
 """
-from .convert import convert, tables, cols16, stream, array_digest  # noqa: F401
+from .convert import convert, tables, cols16, cols8, stream, array_digest  # noqa: F401
 from .model import random_gpt2, prompt_ids, GPT2_SHAPE  # noqa: F401
 from .layout import layout, load_layout, bank_names, rewire  # noqa: F401
 from . import pythia  # noqa: F401
@@ -17,7 +17,7 @@ from . import refs  # noqa: F401
 
 def __getattr__(name):
     # the ctypes binding is loaded on first use so that CPU-only callers never need the HIP runtime
-    if name in ("Machine", "Tables", "Plate", "lib", "LIB_PATH", "SmError", "stages", "check", "profile_stages",
+    if name in ("Machine", "Tables", "Plate", "Plate8", "NarrowCache", "lib", "LIB_PATH", "SmError", "stages", "check", "profile_stages",
                 "kernel_times"):
         from . import machine
         return getattr(machine, name)

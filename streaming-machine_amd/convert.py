@@ -57,6 +57,16 @@ def cols16(W: np.ndarray):
     return q.astype(np.int16), e
 
 
+def cols8(W: np.ndarray):
+    """int8 weights, one power of two per column: cols16's rule at 8 bits (the digits of Plate8)."""
+    mx = np.maximum(np.abs(W).max(axis=0), 1e-30)
+    e = _ceil_log2(mx / 127)
+    q = np.round(W / np.exp2(e.astype(np.float64))[None, :]).astype(np.int64)
+    if np.abs(q).max() > 127:
+        raise ValueError("cols8: a weight does not fit 8 bits")
+    return q.astype(np.int8), e
+
+
 def stream(v: np.ndarray) -> np.ndarray:
     """Whole numbers at the stream's scale 2^-16 (base2_convert.py:28)."""
     return np.round(np.asarray(v, dtype=np.float64) * 2.0 ** ES).astype(np.int64)

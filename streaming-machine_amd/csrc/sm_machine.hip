@@ -26,8 +26,10 @@
 #include <cxxabi.h>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
+#include <type_traits>
 #include <vector>
 
 static thread_local std::string g_err;
@@ -2440,3 +2442,6 @@ extern "C" int sm_plate_product(const sm_plate* p, const int64_t* x16, int64_t* 
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
+
+// operators in few bits: their kernels and entry points
+#include "sm_narrow.hip"

@@ -1,0 +1,870 @@
+// Operators in few bits: plates of 8-bit digits (sm_plate8_*), a cache of 4 or 8-bit digits and the attention over it
+// (sm_narrow_*).  Kernels first, then their entry points.
+//
+// A row's digits of b bits (the machine's to16, base2.py:24-27, at b bits):
+//     sh = max(bitlen(OR |x|) - (b - 1), 0),   digit = clamp(rsh(x, sh), -2^(b-1), 2^(b-1) - 1)
+// worth digit 2^sh each at the row's own scale; sh is the row's level, kept in one byte (0 .. 60).
+//
+// Digits that the matrix units contract stand in the operands' order of v_mfma_i32_16x16x64_i8 (lane l: row or column
+// l % 16, bytes k = 16 (l / 16) + b), so an operand is one 16-byte load a lane, no lane's bytes are moved between lanes
+// and a wave's loads are 1 KB in a row.
+#define NTHREADS 256
+
+// x 2^-s rounded half up without the sum that wraps near 2^63 (s in 0 .. 63)
+SMD i64 rsh_round(i64 x, int s) { return s > 0 ? (x >> s) + ((x >> (s - 1)) & 1) : x; }
+SMD int digit_level(u64 orr, int bits) {
+    const int top = bitlen_u(orr);
+    return top > bits - 1 ? top - (bits - 1) : 0;
+}
+SMD int digit_of(i64 x, int sh, int bits) {
+    const i64 v = rsh_round(x, sh), hi = (1 << (bits - 1)) - 1;
+    return (int)(v > hi ? hi : v < -hi - 1 ? -hi - 1 : v);
+}
+SMD u64 mag64(i64 x) { return x < 0 ? (u64)0 - (u64)x : (u64)x; }
+// the OR over a wave of 64-bit values, in every lane
+SMD u64 wave_or_u64(u64 v) { return (u64)wave_or64((i64)v); }
+
+// ---------------------------------------------------------------------------------------------------------
+// the product with 8-bit digits
+struct Narrow8Args {
+    const signed char* W;        // [column tiles of 16][K / 64][lane][16]
+    const int* we; const i64* wb;
+    int nin, K, N;               // inputs, inputs up to a multiple of 64, columns
+    const i64* X; i64 ldx; int rows;
+    signed char* lights;         // [row tiles of 16][K / 64][lane][16]
+    int* level;                  // [rows] the rows' sh (ex = sh - 16)
+    i64* out; i64 ldo;
+};
+
+// one block a row: the row's level, then its digits in the operand's order (four in a row a thread).  Rows of up to
+// 8,192 values are held in registers between the two passes, longer ones are read again.
+__global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
+    constexpr int HOLD = 8;
+    __shared__ u64 wor[NTHREADS / 64];
+    const int r = blockIdx.x, tid = threadIdx.x, quads = a.K / 4;
+    const i64* x = a.X + (i64)r * a.ldx;
+    auto load = [&](int q, i64 v[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = 4 * q + i < a.nin ? x[4 * q + i] : 0;
+    };
+    i64 held[HOLD][4];
+    u64 orr = 0;
+#pragma unroll
+    for (int s = 0; s < HOLD; s++) {
+        const int q = tid + s * NTHREADS;
+        if (q < quads) {
+            load(q, held[s]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) orr |= mag64(held[s][i]);
+        }
+    }
+    for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
+        i64 v[4];
+        load(q, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) orr |= mag64(v[i]);
+    }
+    orr = wave_or_u64(orr);
+    if ((tid & 63) == 0) wor[tid >> 6] = orr;
+    __syncthreads();
+    orr = 0;
+#pragma unroll
+    for (int i = 0; i < NTHREADS / 64; i++) orr |= wor[i];
+    const int sh = digit_level(orr, 8);
+    if (tid == 0) a.level[r] = sh;
+    signed char* o = a.lights + (i64)(r >> 4) * a.K * 16 + (r & 15) * 16;
+    auto store = [&](int q, const i64 v[4]) {
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (unsigned)(digit_of(v[i], sh, 8) & 255) << (8 * i);
+        const int k = 4 * q;
+        *reinterpret_cast<unsigned*>(o + (i64)(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 15)) = w;
+    };
+#pragma unroll
+    for (int s = 0; s < HOLD; s++)
+        if (tid + s * NTHREADS < quads) store(tid + s * NTHREADS, held[s]);
+    for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
+        i64 v[4];
+        load(q, v);
+        store(q, v);
+    }
+}
+
+SMD v4i mfma8(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+// rsh(pile, -(e + ex + 16)) + b
+SMD i64 narrow_out(int pile, int we, int sh, i64 wb) {
+    const int s = -(we + sh);
+    return wadd(s > 0 ? rsh_round(pile, min(s, 63)) : shl(pile, -s), wb);
+}
+
+// RT row tiles by CT column tiles a wave, the inputs split over KW of a block's four waves and their piles added
+template <int RT, int CT, int KW>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
+    constexpr int CG = 4 / KW, TILES = RT * CT;
+    __shared__ v4i part[4][TILES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ks = wave % KW, cg = wave / KW;
+    const int kbs = a.K / 64, per = (kbs + KW - 1) / KW, k0 = ks * per, k1 = min(kbs, k0 + per);
+    const int nt = (a.N + 15) / 16, ct0 = (blockIdx.x * CG + cg) * CT, rt0 = blockIdx.y * RT, rts = (a.rows + 15) / 16;
+    const v4i *wp[CT], *lp[RT];
+#pragma unroll
+    for (int c = 0; c < CT; c++) wp[c] = reinterpret_cast<const v4i*>(a.W + (i64)min(ct0 + c, nt - 1) * a.K * 16) + lane;
+#pragma unroll
+    for (int r = 0; r < RT; r++) lp[r] = reinterpret_cast<const v4i*>(a.lights + (i64)min(rt0 + r, rts - 1) * a.K * 16) + lane;
+    v4i acc[RT][CT] = {};
+#pragma unroll 4
+    for (int k = k0; k < k1; k++) {
+        v4i w[CT], x[RT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) w[c] = wp[c][k * 64];
+#pragma unroll
+        for (int r = 0; r < RT; r++) x[r] = lp[r][k * 64];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) acc[r][c] = mfma8(x[r], w[c], acc[r][c]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int c = 0; c < CT; c++) part[wave][r * CT + c][lane] = acc[r][c];
+    __syncthreads();
+    for (int t = ks; t < TILES; t += KW) {       // the tiles' piles, shared out over the inputs' waves
+        v4i p = part[cg * KW][t][lane];
+#pragma unroll
+        for (int i = 1; i < KW; i++) p += part[cg * KW + i][t][lane];
+        const int col = (ct0 + t % CT) * 16 + (lane & 15);
+        if (col >= a.N) continue;
+        const int we = a.we[col];
+        const i64 wb = a.wb[col];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = (rt0 + t / CT) * 16 + 4 * (lane >> 4) + i;
+            if (row < a.rows) a.out[(i64)row * a.ldo + col] = narrow_out(p[i], we, a.level[row], wb);
+        }
+    }
+}
+
+// an input-major int8 [nin][nout] array into the operand's order (zeros past nin and past nout)
+__global__ __launch_bounds__(NTHREADS) void k_narrow_plate(const signed char* w, int nin, int nout, int K, signed char* W, i64 quads) {
+    for (i64 q = (i64)blockIdx.x * NTHREADS + threadIdx.x; q < quads; q += (i64)gridDim.x * NTHREADS) {
+        const i64 o = q * 4;                                     // [tile][K / 64][lane][16]
+        const int b = (int)(o & 15), lane = (int)(o >> 4) & 63;
+        const i64 t = o >> 10;
+        const int kbs = K / 64, k = (int)(t % kbs) * 64 + (lane >> 4) * 16 + b, col = (int)(t / kbs) * 16 + (lane & 15);
+        unsigned v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (k + i < nin && col < nout) v |= (unsigned)(unsigned char)w[(i64)(k + i) * nout + col] << (8 * i);
+        *reinterpret_cast<unsigned*>(W + o) = v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the cache.  Each (stream, head) holds tiles of 64 positions: the key digits, the value digits, 64 key levels, 64 value
+// levels (wide: the head's row up to 64, 128 or 256 digits, zeros past its dimension).
+//   keys    [wide / 16 or 32][64 positions][16 bytes]: byte j is dimension 16 c + j; of 4 bits dimension 32 c + j in its low
+//           half and 32 c + 16 + j in its high one
+//   values  [wide / 16][4 g][16 m][16 bytes]: dimension 16 c + m, byte 4 t + r position 16 t + 4 g + r; of 4 bits
+//           [wide / 32][4 g][16 m][2 h][8 bytes]: dimension 32 c + 16 h + m, byte 4 t + r position 16 t + 4 g + r (t 0, 1) in
+//           its low half and the position 32 further in its high one
+// A key operand (64 dimensions of 16 positions) and a value operand (64 positions of 16 dimensions) are then loads of 8 or
+// 16 bytes a lane in the operand's order; the positions' order within a value operand is the order in which a score
+// accumulator holds them (register r of lane group g of tile t), so weights need no exchange where scores stand
+// position-major.  A position's key bytes are its own; its value bytes are shared with the position 32 further at 4 bits.
+struct NarrowShape { int streams, heads, dim, wide, ctx, bits, tiles; };
+SMD i64 narrow_half(const NarrowShape& s) { return (i64)s.wide * 8 * s.bits; }                   // bytes of a tile's keys
+SMD i64 narrow_tile(const NarrowShape& s) { return 2 * narrow_half(s) + 128; }
+SMD char* narrow_at(char* buf, const NarrowShape& s, int stream, int head, int tile) {
+    return buf + (((i64)stream * s.heads + head) * s.tiles + tile) * narrow_tile(s);
+}
+
+struct NarrowRows {
+    NarrowShape s; char* buf;
+    const i64* k; const i64* v; i64* k2; i64* v2;
+    i64 row_stride, stream_stride; int rows;
+    const int* start; const int* count;
+};
+// the rows of a call that are in the cache's range: [lo, hi) of its `rows`
+SMD void narrow_range(const int* start, const int* count, int stream, int rows, int ctx, i64& p0, i64& lo, i64& hi) {
+    p0 = start[stream];
+    hi = count ? min(max(count[stream], 0), rows) : rows;
+    lo = p0 < 0 ? -p0 : 0;
+    hi = min(hi, (i64)ctx - p0);
+}
+
+// a block a (tile, head, stream): its rows' levels and digits (a wave a row) through LDS, then whole 16-byte units; a
+// unit of values is read first where it also holds positions that the call does not write
+template <int BITS, int WIDE>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
+    constexpr int PER = WIDE / 64;
+    __shared__ __attribute__((aligned(16))) signed char kd[64][WIDE + 4], vd[64][WIDE + 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, stream = blockIdx.z;
+    i64 p0, lo, hi;
+    narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
+    if (lo >= hi) return;
+    const i64 first = p0 + lo, last = p0 + hi - 1;                // positions written
+    const i64 tile = first / 64 + blockIdx.x;
+    if (tile > last / 64) return;
+    const int b0 = (int)max(first - tile * 64, (i64)0), b1 = (int)min(last - tile * 64, (i64)63);    // within the tile
+    char* base = narrow_at(a.buf, a.s, stream, head, (int)tile);
+    char* lev = base + 2 * narrow_half(a.s);
+    for (int b = b0 + wave; b <= b1; b += NTHREADS / 64) {
+        const i64 row = tile * 64 + b - p0, at = stream * a.stream_stride + row * a.row_stride + (i64)head * a.s.dim;
+        i64 xk[PER], xv[PER];
+        u64 ok = 0, ov = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int d = lane + 64 * i;
+            xk[i] = d < a.s.dim ? a.k[at + d] : 0;
+            xv[i] = d < a.s.dim ? a.v[at + d] : 0;
+            ok |= mag64(xk[i]);
+            ov |= mag64(xv[i]);
+        }
+        const int sk = digit_level(wave_or_u64(ok), BITS), sv = digit_level(wave_or_u64(ov), BITS);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            kd[b][lane + 64 * i] = (signed char)digit_of(xk[i], sk, BITS);
+            vd[b][lane + 64 * i] = (signed char)digit_of(xv[i], sv, BITS);
+        }
+        if (lane == 0) { lev[b] = (char)sk; lev[64 + b] = (char)sv; }
+    }
+    __syncthreads();
+    constexpr int UNITS = WIDE * BITS / 128;                     // 16-byte units a position, or a dimension's 64 / 4
+    for (int i = tid; i < UNITS * 64; i += NTHREADS) {
+        const int c = i >> 6, b = i & 63;
+        if (b < b0 || b > b1) continue;
+        unsigned w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            w[q] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned v = BITS == 8 ? (unsigned)kd[b][16 * c + 4 * q + j] & 255u
+                    : ((unsigned)kd[b][32 * c + 4 * q + j] & 15u) | ((unsigned)kd[b][32 * c + 16 + 4 * q + j] & 15u) << 4;
+                w[q] |= v << (8 * j);
+            }
+        }
+        *reinterpret_cast<v4i*>(base + (i64)i * 16) = v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    }
+    char* vbase = base + narrow_half(a.s);
+    for (int i = tid; i < UNITS * 64; i += NTHREADS) {
+        const int c = i >> 6, g = (i >> 4) & 3, m = i & 15;
+        // the unit's positions 16 t + 4 g + r: which of them the call writes
+        unsigned in = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int p = 16 * (j >> 2) + 4 * g + (j & 3);
+            in |= (p >= b0 && p <= b1 ? 1u : 0u) << j;
+        }
+        if (!in) continue;
+        v4i* u = reinterpret_cast<v4i*>(vbase + (i64)i * 16);
+        v4i old = {};
+        if (in != 0xFFFFu) old = *u;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            unsigned w = 0, keep = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (BITS == 8) {
+                    const int p = 16 * q + 4 * g + j;
+                    w |= ((unsigned)vd[p][16 * c + m] & 255u) << (8 * j);
+                    keep |= (in >> (4 * q + j) & 1 ? 0u : 255u) << (8 * j);
+                } else {
+                    const int t = q & 1, p = 16 * t + 4 * g + j, d = 32 * c + 16 * (q >> 1) + m;
+                    w |= (((unsigned)vd[p][d] & 15u) | ((unsigned)vd[p + 32][d] & 15u) << 4) << (8 * j);
+                    keep |= ((in >> (4 * t + j) & 1 ? 0u : 15u) | (in >> (4 * t + 8 + j) & 1 ? 0u : 240u)) << (8 * j);
+                }
+            }
+            old[q] = (int)((w & ~keep) | ((unsigned)old[q] & keep));
+        }
+        *u = old;
+    }
+}
+
+// a thread a (row, head, dimension)
+template <int BITS>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_read(NarrowRows a) {
+    const int stream = blockIdx.z, hd = a.s.heads * a.s.dim;
+    i64 p0, lo, hi;
+    narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
+    const i64 n = (hi - lo) * hd;
+    for (i64 i = (i64)blockIdx.x * NTHREADS + threadIdx.x; i < n; i += (i64)gridDim.x * NTHREADS) {
+        const i64 row = lo + i / hd, p = p0 + row;
+        const int h = (int)(i % hd) / a.s.dim, d = (int)(i % hd) % a.s.dim, b = (int)(p & 63), j = 4 * (b >> 4) + (b & 3), g = (b >> 2) & 3;
+        const char* base = narrow_at(a.buf, a.s, stream, h, (int)(p >> 6));
+        const char* vbase = base + narrow_half(a.s);
+        const unsigned char* lev = reinterpret_cast<const unsigned char*>(vbase + narrow_half(a.s));
+        int kv, vv;
+        if (BITS == 8) {
+            kv = (signed char)base[(d >> 4) * 1024 + b * 16 + (d & 15)];
+            vv = (signed char)vbase[(d >> 4) * 1024 + (16 * g + (d & 15)) * 16 + j];
+        } else {
+            const int kb = (signed char)base[(d >> 5) * 1024 + b * 16 + (d & 15)];
+            const int vb = (signed char)vbase[(d >> 5) * 1024 + (16 * g + (d & 15)) * 16 + 8 * (d >> 4 & 1) + (j & 7)];
+            kv = d & 16 ? kb >> 4 : (int)((unsigned)kb << 28) >> 28;
+            vv = j & 8 ? vb >> 4 : (int)((unsigned)vb << 28) >> 28;
+        }
+        const i64 at = stream * a.stream_stride + row * a.row_stride + (i64)h * a.s.dim + d;
+        a.k2[at] = shl(kv, lev[b]);
+        a.v2[at] = shl(vv, lev[64 + b]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// attention over the cache.  A row (stream, row t, query head) at position p = start + t sees positions 0 .. p of its key
+// head.  With q's 8-bit digits at level eq (q 2^(F / 65536) = q8 2^eq, a score's scale folded in through the power's fine
+// part, base2.py:50-53) and ARR the arrivals (base2.py:97):
+//   sc_i = clamp(rsh(sum_d q8_d k_id, -(eq + level_i - 16 + 10)), +-2^30)
+//   chunk j (positions 256 j ..):  m_j = max sc, E_j = max value level (of the positions seen),
+//       u_i = rsh(ARR[m_j - sc_i], 2), A_j = sum u_i, w_i = rsh(u_i, E_j - level_i), N_j = rsh(sum_i w_i v_i, 8)
+//   row:  M = max m_j, E = max E_j, f_j = ARR[M - m_j], A = sum rsh(A_j f_j, 24), N = sum rsh(N_j f_j, 24 + E - E_j)
+//   out = power(N, (E + 8) 65536 - log2fix(A))
+// Sums of whole numbers: no split of the positions over waves or blocks changes them.  Up to 256 positions this is
+// base2.py:93-99 on the digits.
+#define NCHUNK 256
+
+struct NarrowAtt {
+    NarrowShape s; const char* buf;
+    int group, rows, R, J;       // query heads a key head, rows a stream, rows x group, chunks
+    const i64* q; i64 q_row, q_stream; i64* out; i64 o_row, o_stream;
+    const int* start; const int* count; int span; int F;
+    signed char* q8;             // [streams][heads][R][wide]
+    int* eq; int* pos;           // [streams][heads][R] the digits' level; the row's position, -1 a row that is not there
+    float* pm; int* pA; int* pE; int* pN;   // [streams][heads][J][R] each chunk's m_j, A_j, E_j and (x wide) N_j
+    Tables tb;
+};
+
+// one wave a (row, query head): q's digits
+__global__ __launch_bounds__(NTHREADS) void k_narrow_q(NarrowAtt a) {
+    const int lane = threadIdx.x & 63, stream = blockIdx.z, q_heads = a.s.heads * a.group;
+    const int i = blockIdx.x * (NTHREADS / 64) + (threadIdx.x >> 6);
+    if (i >= a.rows * q_heads) return;
+    const int t = i / q_heads, hq = i % q_heads, h = hq / a.group, rho = t * a.group + hq % a.group;
+    const i64 slot = ((i64)stream * a.s.heads + h) * a.R + rho;
+    const i64 p = (i64)a.start[stream] + t;
+    const bool here = t < (a.count ? a.count[stream] : a.rows) && p >= 0 && p < a.span;
+    if (lane == 0) a.pos[slot] = here ? (int)p : -1;
+    i64 x[4];
+    u64 o = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int d = lane + 64 * j;
+        x[j] = here && d < a.s.dim ? a.q[stream * a.q_stream + t * a.q_row + (i64)hq * a.s.dim + d] : 0;
+        o |= mag64(x[j]);
+    }
+    const int s16 = digit_level(wave_or_u64(o), 16);
+    const i64 e = a.tb.EXP2[a.F & 0xFFFF];
+    o = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        x[j] = rsh_round(x[j], s16) * e;
+        o |= mag64(x[j]);
+    }
+    const int s8 = digit_level(wave_or_u64(o), 8);
+    if (lane == 0) a.eq[slot] = s16 - 16 + (a.F >> 16) - 16 + s8;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (lane + 64 * j < a.s.wide) a.q8[slot * a.s.wide + lane + 64 * j] = (signed char)digit_of(x[j], s8, 8);
+}
+
+// 4-bit digits of a dword as bytes of 16 times the digit (the low halves, the high halves)
+SMD int nib_lo(int x) { return (int)((unsigned)x << 4 & 0xF0F0F0F0u); }
+SMD int nib_hi(int x) { return (int)((unsigned)x & 0xF0F0F0F0u); }
+template <int CTRL> SMD int dpp_rot(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false); }
+// a row's total over the lanes that hold it (all 16 columns; with GR rows a tile also the lane groups 16 GR / 4 apart),
+// in every one of them
+template <int GR, class T, class F>
+SMD T row_total(T v, F op) {
+    auto rot = [&](auto c) { v = op(v, __builtin_bit_cast(T, dpp_rot<decltype(c)::value>(__builtin_bit_cast(int, v)))); };
+    rot(std::integral_constant<int, 0x128>());
+    rot(std::integral_constant<int, 0x124>());
+    rot(std::integral_constant<int, 0x122>());
+    rot(std::integral_constant<int, 0x121>());
+    if (GR <= 4) v = op(v, __shfl_xor(v, 16, 64));
+    if (GR <= 8) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+
+// the key operands of 16 positions from `sub`: DK x (64 dimensions)
+template <int BITS, int DK>
+SMD void key_operands(const char* keys, int sub, int lane, v4i out[DK]) {
+    const int n = lane & 15, g = lane >> 4, p = 16 * sub + n;
+    if constexpr (BITS == 8) {
+#pragma unroll
+        for (int u = 0; u < DK; u++) out[u] = *reinterpret_cast<const v4i*>(keys + (4 * u + g) * 1024 + p * 16);
+    } else if constexpr (DK == 1) {
+        const int2 x = *reinterpret_cast<const int2*>(keys + (g >> 1) * 1024 + p * 16 + 8 * (g & 1));
+        out[0] = v4i{nib_lo(x.x), nib_lo(x.y), nib_hi(x.x), nib_hi(x.y)};
+    } else {
+#pragma unroll
+        for (int u = 0; u < DK / 2; u++) {
+            const v4i x = *reinterpret_cast<const v4i*>(keys + (4 * u + g) * 1024 + p * 16);
+            out[2 * u] = v4i{nib_lo(x[0]), nib_lo(x[1]), nib_lo(x[2]), nib_lo(x[3])};
+            out[2 * u + 1] = v4i{nib_hi(x[0]), nib_hi(x[1]), nib_hi(x[2]), nib_hi(x[3])};
+        }
+    }
+}
+// q's digits in the same order (row: the row's digits)
+template <int BITS, int DK>
+SMD void q_operands(const signed char* row, int g, v4i out[DK]) {
+#pragma unroll
+    for (int u = 0; u < DK; u++) {
+        if constexpr (BITS == 4 && DK == 1) {
+            const int2 x = *reinterpret_cast<const int2*>(row + 32 * (g >> 1) + 8 * (g & 1)),
+                       y = *reinterpret_cast<const int2*>(row + 32 * (g >> 1) + 8 * (g & 1) + 16);
+            out[u] = v4i{x.x, x.y, y.x, y.y};
+        } else {
+            out[u] = *reinterpret_cast<const v4i*>(row + (BITS == 8 ? 64 * u + 16 * g : 32 * (4 * (u / 2) + g) + 16 * (u % 2)));
+        }
+    }
+}
+// the value operands of one unit of a tile: 16 dimensions (8 bits) or twice 16 (4 bits)
+template <int BITS>
+SMD void value_operands(v4i x, v4i out[8 / BITS]) {
+    if constexpr (BITS == 8) out[0] = x;
+    else {
+        out[0] = v4i{nib_lo(x[0]), nib_lo(x[1]), nib_hi(x[0]), nib_hi(x[1])};
+        out[1] = v4i{nib_lo(x[2]), nib_lo(x[3]), nib_hi(x[2]), nib_hi(x[3])};
+    }
+}
+
+// A wave a (chunk, tile of GR rows, key head, stream).  Scores: A = q, B = keys, so a lane is a position.  With fewer than
+// 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position tiles add into
+// one accumulator: every lane then holds a score that is wanted.  Weights: byte planes through the wave's LDS, their
+// planes stacked as rows of one operand (3 GR rows in NM operands).
+template <int BITS, int DK, int GR>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblocks) {
+    constexpr int NA = GR / 4, PT = 16 / GR, NM = (3 * GR + 15) / 16, DT = 4 * DK, VU = 8 / BITS;
+    constexpr float NONE = -3e9f;
+    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][NM * 16 * 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int j = (blockIdx.x % jblocks) * (NTHREADS / 64) + wave, rt = blockIdx.x / jblocks, h = blockIdx.y, stream = blockIdx.z;
+    const i64 head = (i64)stream * a.s.heads + h;
+    // the lane's rows
+    int row[4], pos[4];
+    int er[4];
+    int phi = -1, plo = 1 << 30;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        row[r] = rt * GR + (4 * g + r) % GR;
+        const i64 slot = head * a.R + min(row[r], a.R - 1);
+        pos[r] = a.pos[slot];
+        er[r] = a.eq[slot] - 6 - (BITS == 4 ? 4 : 0);
+        phi = max(phi, pos[r]);
+        plo = min(plo, pos[r]);
+    }
+    phi = max(phi, __shfl_xor(phi, 16, 64)); phi = max(phi, __shfl_xor(phi, 32, 64));
+    plo = min(plo, __shfl_xor(plo, 16, 64)); plo = min(plo, __shfl_xor(plo, 32, 64));
+    phi = __builtin_amdgcn_readfirstlane(phi);
+    plo = __builtin_amdgcn_readfirstlane(plo);
+    const int c0 = j * NCHUNK;
+    if (j >= a.J || c0 > phi) return;
+    const bool whole = c0 + NCHUNK - 1 <= plo;
+    // q: operand row m holds row m % GR of the tile, for the position tiles t' = m / GR alone
+    v4i q[PT][DK];
+    {
+        const int m = n;
+        v4i x[DK];
+        q_operands<BITS, DK>(a.q8 + (head * a.R + min(rt * GR + m % GR, a.R - 1)) * a.s.wide, g, x);
+#pragma unroll
+        for (int t = 0; t < PT; t++)
+#pragma unroll
+            for (int u = 0; u < DK; u++) q[t][u] = m / GR == t ? x[u] : v4i{};
+    }
+    const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
+    const char* base = a.buf + head * a.s.tiles * tile_bytes;
+    const int last_tile = phi / 64;
+    float sc[4][GR];
+    int vl[4][NA];
+    float mr[4];
+    int Er[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) { mr[r] = NONE; Er[r] = 0; }
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const char* tp = base + (i64)min(4 * j + t, last_tile) * tile_bytes;
+        const unsigned char* lev = reinterpret_cast<const unsigned char*>(tp + 2 * half);
+        v4i acc[NA] = {};
+#pragma unroll
+        for (int sub = 0; sub < 4; sub++) {
+            v4i k[DK];
+            key_operands<BITS, DK>(tp, sub, lane, k);
+#pragma unroll
+            for (int u = 0; u < DK; u++) acc[sub / PT] = mfma8(q[sub % PT][u], k[u], acc[sub / PT]);
+        }
+#pragma unroll
+        for (int x = 0; x < NA; x++) {
+            const int at = 16 * (x * PT + 4 * g / GR) + n, i = c0 + 64 * t + at;
+            const int kl = lev[at];
+            vl[t][x] = lev[64 + at];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                // dot 2^-s + 1/2 is exact in float: dot has at most 23 bits, and where s <= 0 no half is needed
+                const float v = floorf(ldexpf((float)acc[x][r], er[r] + kl) + 0.5f);
+                float w = fminf(fmaxf(v, -1073741824.f), 1073741824.f);
+                if (!whole && i > pos[r]) w = NONE;
+                sc[t][4 * x + r] = w;
+                mr[r] = fmaxf(mr[r], w);
+                Er[r] = max(Er[r], whole || i <= pos[r] ? vl[t][x] : 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        mr[r] = row_total<GR>(mr[r], [](float x, float y) { return fmaxf(x, y); });
+        Er[r] = row_total<GR>(Er[r], [](int x, int y) { return max(x, y); });
+    }
+    v4i C[NM][DT] = {};
+    int A[4] = {};
+    unsigned char* wb = wbuf[wave];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const char* vp = base + (i64)min(4 * j + t, last_tile) * tile_bytes + half;
+        v4i v[DT / VU];
+#pragma unroll
+        for (int c = 0; c < DT / VU; c++) v[c] = *reinterpret_cast<const v4i*>(vp + c * 1024 + lane * 16);
+#pragma unroll
+        for (int x = 0; x < NA; x++) {
+            const int T = x * PT + 4 * g / GR;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float d = fminf(mr[r] - sc[t][4 * x + r], (float)a.tb.alen);
+                const int i = (int)d;
+                const int u = i < a.tb.alen ? (a.tb.ARR[i] + 2) >> 2 : 0;
+                A[r] += u;
+                const int w = (((u << 1) >> min(Er[r] - vl[t][x], 31)) + 1) >> 1;
+                const unsigned b = ((unsigned)w + 0x808080u) ^ 0x808080u;
+                const int row0 = (4 * g + r) % GR, o = 16 * (n >> 2) + 4 * T + (n & 3);
+                wb[row0 * 64 + o] = (unsigned char)b;
+                wb[(GR + row0) * 64 + o] = (unsigned char)(b >> 8);
+                wb[(2 * GR + row0) * 64 + o] = (unsigned char)(b >> 16);
+            }
+        }
+        v4i w[NM];
+#pragma unroll
+        for (int k = 0; k < NM; k++) w[k] = *reinterpret_cast<const v4i*>(wb + (16 * k + n) * 64 + 16 * g);
+#pragma unroll
+        for (int c = 0; c < DT / VU; c++) {
+            v4i o[VU];
+            value_operands<BITS>(v[c], o);
+#pragma unroll
+            for (int y = 0; y < VU; y++)
+#pragma unroll
+                for (int k = 0; k < NM; k++) C[k][c * VU + y] = mfma8(w[k], o[y], C[k][c * VU + y]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) A[r] = row_total<GR>(A[r], [](int x, int y) { return x + y; });
+    const i64 slot0 = (head * a.J + j) * a.R;
+    if (n == 0 && 4 * g < GR)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (row[r] < a.R) { a.pm[slot0 + row[r]] = mr[r]; a.pA[slot0 + row[r]] = A[r]; a.pE[slot0 + row[r]] = Er[r]; }
+#pragma unroll
+    for (int c = 0; c < DT; c++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            int n0, n1, n2;
+            if constexpr (GR == 16) { n0 = C[0][c][r]; n1 = C[1][c][r]; n2 = C[2][c][r]; }
+            else if constexpr (GR == 8) { n0 = C[0][c][r]; n1 = __shfl_xor(n0, 32, 64); n2 = C[1][c][r]; }
+            else { n0 = C[0][c][r]; n1 = __shfl_xor(n0, 16, 64); n2 = __shfl_xor(n0, 32, 64); }
+            // rsh(n0 + 256 n1 + 65536 n2, 8), the digits of 4 bits 16 times their value
+            const int q8 = n1 + (n2 << 8);
+            const int N = BITS == 8 ? q8 + ((n0 + 128) >> 8) : (q8 + ((n0 + 2048) >> 8)) >> 4;
+            if (4 * g < GR && row[r] < a.R) a.pN[(slot0 + row[r]) * a.s.wide + 16 * c + n] = N;
+        }
+}
+
+// a block a row: its chunks joined
+__global__ __launch_bounds__(NTHREADS) void k_narrow_join(NarrowAtt a) {
+    __shared__ float sm[4];
+    __shared__ int se[4];
+    __shared__ i64 sa[4];
+    __shared__ i64 sn[NTHREADS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rho = blockIdx.x, h = blockIdx.y, stream = blockIdx.z;
+    const i64 head = (i64)stream * a.s.heads + h;
+    const int p = a.pos[head * a.R + rho];
+    if (p < 0) return;
+    const int J = p / NCHUNK + 1;
+    float M = -3e9f;
+    int E = 0;
+    for (int j = tid; j < J; j += NTHREADS) {
+        const i64 s = (head * a.J + j) * a.R + rho;
+        M = fmaxf(M, a.pm[s]);
+        E = max(E, a.pE[s]);
+    }
+    for (int o = 1; o < 64; o <<= 1) { M = fmaxf(M, __shfl_xor(M, o, 64)); E = max(E, __shfl_xor(E, o, 64)); }
+    if (lane == 0) { sm[wave] = M; se[wave] = E; }
+    __syncthreads();
+    for (int i = 0; i < 4; i++) { M = fmaxf(M, sm[i]); E = max(E, se[i]); }
+    auto f_of = [&](i64 s) {
+        const float d = M - a.pm[s];
+        return d < (float)a.tb.alen ? (i64)a.tb.ARR[(int)d] : 0;
+    };
+    i64 A = 0;
+    for (int j = tid; j < J; j += NTHREADS) {
+        const i64 s = (head * a.J + j) * a.R + rho;
+        A += rsh_round(a.pA[s] * f_of(s), 24);
+    }
+    A = wave_reduce64(A, OpAdd());
+    if (lane == 0) sa[wave] = A;
+    const int wide = a.s.wide, d = tid % wide, slice = tid / wide, slices = NTHREADS / wide;
+    i64 N = 0;
+    for (int j = slice; j < J; j += slices) {
+        const i64 s = (head * a.J + j) * a.R + rho;
+        N += rsh_round(a.pN[s * wide + d] * f_of(s), min(24 + E - a.pE[s], 63));
+    }
+    sn[tid] = N;
+    __syncthreads();
+    if (tid >= a.s.dim) return;
+    A = sa[0] + sa[1] + sa[2] + sa[3];
+    for (int i = 1; i < slices; i++) N += sn[i * wide + d];
+    const int t = rho / a.group, hq = h * a.group + rho % a.group;
+    a.out[stream * a.o_stream + t * a.o_row + (i64)hq * a.s.dim + d] = power(N, ((i64)E + 8) * 65536 - log2fix(A, a.tb), a.tb);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// entry points
+
+// The device that holds a call's memory, made current for the call.  Memory that no device holds is refused here, before a
+// kernel reads it.
+struct OnDevice {
+    int was = -1, dev = -1;
+    bool ok = false;
+    explicit OnDevice(const void* p) {
+        hipPointerAttribute_t at{};
+        if (hipPointerGetAttributes(&at, p) != hipSuccess) { (void)hipGetLastError(); return; }
+        if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) return;
+        if (hipGetDevice(&was) != hipSuccess) return;
+        dev = at.device;
+        ok = dev == was || hipSetDevice(dev) == hipSuccess;
+    }
+    ~OnDevice() { if (ok && dev != was) (void)hipSetDevice(was); }
+    OnDevice(const OnDevice&) = delete;
+};
+
+struct sm_plate8 {
+    signed char* W = nullptr; int* e = nullptr; i64* b = nullptr;
+    int nin = 0, nout = 0, K = 0;
+    i64 bytes = 0;
+};
+static void plate8_free(sm_plate8* p) {
+    hfree(p->W); hfree(p->e); hfree(p->b);
+    delete p;
+}
+
+extern "C" int sm_plate8_create(const int8_t* w, const int32_t* e, const int64_t* b, int32_t nin, int32_t nout, sm_plate8** out) {
+    if (!w || !e || !b || !out) return fail(SM_E_ARG, "sm_plate8_create: null argument");
+    if (nin < 1 || nin > SM_PLATE8_NIN || nout < 1 || nout > (1 << 24)) return fail(SM_E_ARG, "sm_plate8_create: nin or nout out of range");
+    for (int32_t i = 0; i < nout; i++)
+        if (e[i] < -1024 || e[i] > 1024) return fail(SM_E_ARG, "sm_plate8_create: a column's power is out of range");
+    sm_plate8* p = new (std::nothrow) sm_plate8();
+    if (!p) return fail(SM_E_OOM, "sm_plate8_create: host memory");
+    p->nin = nin; p->nout = nout; p->K = (nin + 63) / 64 * 64;
+    p->bytes = (i64)((nout + 15) / 16) * 16 * p->K;
+    signed char* raw = nullptr;
+    int rc;
+    auto make = [&]() -> int {
+        if ((rc = dalloc(&p->W, (size_t)p->bytes)) || (rc = dalloc(&p->e, (size_t)nout)) || (rc = dalloc(&p->b, (size_t)nout)) ||
+            (rc = dalloc(&raw, (size_t)nin * nout)))
+            return rc;
+        HIP_TRY(hipMemcpy(raw, w, (size_t)nin * nout, hipMemcpyHostToDevice));
+        HIP_TRY(hipMemcpy(p->e, e, (size_t)nout * 4, hipMemcpyHostToDevice));
+        HIP_TRY(hipMemcpy(p->b, b, (size_t)nout * 8, hipMemcpyHostToDevice));
+        const i64 quads = p->bytes / 4;
+        const unsigned blocks = (unsigned)std::min<i64>((quads + NTHREADS - 1) / NTHREADS, 1 << 16);
+        launch(false, "plate8.lay", k_narrow_plate, dim3(blocks), dim3(NTHREADS), 0, nullptr, (const signed char*)raw, (int)nin, (int)nout, p->K, p->W, quads);
+        HIP_TRY(hipGetLastError());
+        HIP_TRY(hipStreamSynchronize(nullptr));
+        return SM_OK;
+    };
+    rc = make();
+    hfree(raw);
+    if (rc) { plate8_free(p); return rc; }
+    *out = p;
+    return SM_OK;
+}
+extern "C" int sm_plate8_destroy(sm_plate8* p) {
+    if (p) {
+        OnDevice on(p->W);
+        (void)hipDeviceSynchronize();
+        plate8_free(p);
+    }
+    return SM_OK;
+}
+extern "C" int64_t sm_plate8_bytes(const sm_plate8* p) { return p ? p->bytes : 0; }
+
+static i64 up256(i64 n) { return (n + 255) / 256 * 256; }
+static i64 plate8_lights(const sm_plate8* p, int rows) { return up256((i64)((rows + 15) / 16) * 16 * p->K); }
+extern "C" int64_t sm_plate8_work(const sm_plate8* p, int32_t rows) {
+    if (!p || rows < 0) { fail(SM_E_ARG, "sm_plate8_work: arguments"); return SM_E_ARG; }
+    return plate8_lights(p, rows) + up256((i64)rows * 4);
+}
+
+extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x_stride, int32_t rows, int64_t* out,
+                                 int64_t out_stride, void* work, int64_t work_bytes, void* stream) {
+    if (!p) return fail(SM_E_ARG, "sm_plate8_product: null plate");
+    if (rows < 0 || rows > SM_PLATE8_ROWS) return fail(SM_E_ARG, "sm_plate8_product: rows out of range");
+    if (!rows) return SM_OK;
+    if (!X || !out || !work) return fail(SM_E_ARG, "sm_plate8_product: null argument");
+    if (x_stride < p->nin || out_stride < p->nout) return fail(SM_E_ARG, "sm_plate8_product: a row stride is shorter than its row");
+    if (((uintptr_t)X | (uintptr_t)out) & 7 || (uintptr_t)work & 15) return fail(SM_E_ARG, "sm_plate8_product: alignment (rows 8 bytes, work 16)");
+    if (work_bytes < sm_plate8_work(p, rows)) return fail(SM_E_ARG, "sm_plate8_product: the workspace is smaller than sm_plate8_work");
+    OnDevice on(p->W);
+    if (!on.ok) return fail(SM_E_HIP, "sm_plate8_product: the plate's device");
+    Narrow8Args a{};
+    a.W = p->W; a.we = p->e; a.wb = p->b; a.nin = p->nin; a.K = p->K; a.N = p->nout;
+    a.X = (const i64*)X; a.ldx = x_stride; a.rows = rows; a.out = (i64*)out; a.ldo = out_stride;
+    a.lights = static_cast<signed char*>(work);
+    a.level = reinterpret_cast<int*>(static_cast<char*>(work) + plate8_lights(p, rows));
+    hipStream_t s = (hipStream_t)stream;
+    launch(g_kt.stages, "plate8.lights", k_narrow_lights, dim3(rows), dim3(NTHREADS), 0, s, a);
+    const int nt = (a.N + 15) / 16, rts = (rows + 15) / 16;
+    if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
+    else if (rts == 2) launch(g_kt.stages, "plate8.rows", k_narrow_rows<2, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
+    else launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3(nt, (rts + 3) / 4), dim3(NTHREADS), 0, s, a);
+    HIP_TRY(hipGetLastError());
+    return SM_OK;
+}
+
+// ---- the cache
+static int narrow_shape(const sm_narrow* c, NarrowShape& s, const char* who) {
+    const std::string w(who);
+    if (!c) return fail(SM_E_ARG, w + ": null shape");
+    if (c->streams < 1 || c->streams > 65535 || c->heads < 1 || c->heads > 65535) return fail(SM_E_ARG, w + ": streams and heads are 1 .. 65535");
+    if (c->dim < 1 || c->dim > 256) return fail(SM_E_ARG, w + ": a head has 1 .. 256 dimensions");
+    if (c->ctx < 1 || c->ctx > (1 << 24)) return fail(SM_E_ARG, w + ": ctx is 1 .. 2^24");
+    if (c->bits != 4 && c->bits != 8) return fail(SM_E_ARG, w + ": digits of 4 or 8 bits");
+    s.streams = c->streams; s.heads = c->heads; s.dim = c->dim; s.ctx = c->ctx; s.bits = c->bits;
+    s.wide = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+    s.tiles = (c->ctx + 63) / 64;
+    return SM_OK;
+}
+static i64 narrow_tile_bytes(const NarrowShape& s) { return (i64)s.wide * 16 * s.bits + 128; }
+extern "C" int64_t sm_narrow_bytes(const sm_narrow* c) {
+    NarrowShape s;
+    const int rc = narrow_shape(c, s, "sm_narrow_bytes");
+    return rc ? rc : (i64)s.streams * s.heads * s.tiles * narrow_tile_bytes(s);
+}
+
+static int narrow_rows(const sm_narrow* c, const void* buf, const void* k, const void* v, int64_t row_stride, int64_t stream_stride,
+                       int32_t rows, const int32_t* start, NarrowShape& s, const char* who) {
+    const std::string w(who);
+    int rc = narrow_shape(c, s, who);
+    if (rc) return rc;
+    if (rows < 0 || rows > s.ctx) return fail(SM_E_ARG, w + ": rows are 0 .. ctx");
+    if (!rows) return SM_OK;
+    if (!buf || !k || !v || !start) return fail(SM_E_ARG, w + ": null argument");
+    if (row_stride < (int64_t)s.heads * s.dim || stream_stride < 0) return fail(SM_E_ARG, w + ": strides");
+    if ((uintptr_t)buf & 15 || ((uintptr_t)k | (uintptr_t)v) & 7 || (uintptr_t)start & 3) return fail(SM_E_ARG, w + ": alignment (cache 16 bytes, rows 8)");
+    return SM_OK;
+}
+
+extern "C" int sm_narrow_write(const sm_narrow* c, void* buf, const int64_t* k, const int64_t* v, int64_t row_stride,
+                               int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream) {
+    NarrowRows a{};
+    int rc = narrow_rows(c, buf, k, v, row_stride, stream_stride, rows, start, a.s, "sm_narrow_write");
+    if (rc || !rows) return rc;
+    OnDevice on(buf);
+    if (!on.ok) return fail(SM_E_ARG, "sm_narrow_write: the cache is not in a device's memory");
+    a.buf = static_cast<char*>(buf); a.k = (const i64*)k; a.v = (const i64*)v;
+    a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
+    const dim3 grid((unsigned)((rows + 62) / 64 + 1), (unsigned)a.s.heads, (unsigned)a.s.streams);
+    auto go = [&](auto kern) { launch(g_kt.stages, "narrow.write", kern, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a); };
+    if (a.s.bits == 4) a.s.wide == 64 ? go(k_narrow_write<4, 64>) : a.s.wide == 128 ? go(k_narrow_write<4, 128>) : go(k_narrow_write<4, 256>);
+    else a.s.wide == 64 ? go(k_narrow_write<8, 64>) : a.s.wide == 128 ? go(k_narrow_write<8, 128>) : go(k_narrow_write<8, 256>);
+    HIP_TRY(hipGetLastError());
+    return SM_OK;
+}
+
+extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, int64_t* v, int64_t row_stride,
+                              int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream) {
+    NarrowRows a{};
+    int rc = narrow_rows(c, buf, k, v, row_stride, stream_stride, rows, start, a.s, "sm_narrow_read");
+    if (rc || !rows) return rc;
+    OnDevice on(buf);
+    if (!on.ok) return fail(SM_E_ARG, "sm_narrow_read: the cache is not in a device's memory");
+    a.buf = static_cast<char*>(const_cast<void*>(buf)); a.k2 = (i64*)k; a.v2 = (i64*)v;
+    a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
+    const i64 n = (i64)rows * a.s.heads * a.s.dim;
+    const dim3 grid((unsigned)std::min<i64>((n + NTHREADS - 1) / NTHREADS, 4096), 1, (unsigned)a.s.streams);
+    if (a.s.bits == 4) launch(g_kt.stages, "narrow.read", k_narrow_read<4>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
+    else launch(g_kt.stages, "narrow.read", k_narrow_read<8>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError());
+    return SM_OK;
+}
+
+// ---- the attention's workspace: q's digits, the rows' levels and positions, the chunks' partial sums
+struct NarrowWork { i64 q8, eq, pos, pm, pA, pE, pN, bytes; };
+static NarrowWork narrow_work(const NarrowShape& s, int R, int J) {
+    const i64 n = (i64)s.streams * s.heads * R;
+    NarrowWork w{};
+    w.q8 = 0;
+    w.eq = up256(n * s.wide);
+    w.pos = w.eq + up256(n * 4);
+    w.pm = w.pos + up256(n * 4);
+    w.pA = w.pm + up256(n * J * 4);
+    w.pE = w.pA + up256(n * J * 4);
+    w.pN = w.pE + up256(n * J * 4);
+    w.bytes = w.pN + n * J * s.wide * 4;
+    return w;
+}
+static int narrow_att_args(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span, NarrowShape& s, const char* who) {
+    const std::string w(who);
+    int rc = narrow_shape(c, s, who);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads > 65535 || q_heads % s.heads) return fail(SM_E_ARG, w + ": query heads are a multiple of the cache's heads");
+    if (rows < 0 || rows > s.ctx) return fail(SM_E_ARG, w + ": rows are 0 .. ctx");
+    if (span < 1 || span > s.ctx) return fail(SM_E_ARG, w + ": span is 1 .. ctx");
+    if ((i64)rows * q_heads > (1 << 22)) return fail(SM_E_ARG, w + ": rows x query heads are at most 2^22");
+    return SM_OK;
+}
+extern "C" int64_t sm_narrow_work(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span) {
+    NarrowShape s;
+    const int rc = narrow_att_args(c, q_heads, rows, span, s, "sm_narrow_work");
+    return rc ? rc : narrow_work(s, rows * (q_heads / s.heads), (span + NCHUNK - 1) / NCHUNK).bytes;
+}
+
+template <int BITS, int DK>
+static void narrow_split(const NarrowAtt& a, hipStream_t st) {
+    const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, jb = (a.J + 3) / 4;
+    const dim3 grid((unsigned)(jb * ((a.R + gr - 1) / gr)), (unsigned)a.s.heads, (unsigned)a.s.streams);
+    if (gr == 4) launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 4>, grid, dim3(NTHREADS), 0, st, a, jb);
+    else if (gr == 8) launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 8>, grid, dim3(NTHREADS), 0, st, a, jb);
+    else launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 16>, grid, dim3(NTHREADS), 0, st, a, jb);
+}
+
+extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const void* buf, const int64_t* q, int64_t q_row, int64_t q_stream,
+                                int32_t q_heads, int32_t rows, int32_t span, const int32_t* start, const int32_t* count, int32_t scale,
+                                int64_t* out, int64_t out_row, int64_t out_stream, void* work, int64_t work_bytes, void* stream) {
+    NarrowAtt a{};
+    if (!t) return fail(SM_E_ARG, "sm_narrow_attend: null tables");
+    int rc = narrow_att_args(c, q_heads, rows, span, a.s, "sm_narrow_attend");
+    if (rc || !rows) return rc;
+    if (!buf || !q || !start || !out || !work) return fail(SM_E_ARG, "sm_narrow_attend: null argument");
+    const i64 width = (i64)q_heads * a.s.dim;
+    if (q_row < width || out_row < width || q_stream < 0 || out_stream < 0) return fail(SM_E_ARG, "sm_narrow_attend: strides");
+    if (scale < -(64 << 16) || scale > (64 << 16)) return fail(SM_E_ARG, "sm_narrow_attend: the scale's log2 is out of range");
+    if (((uintptr_t)buf | (uintptr_t)work) & 15 || ((uintptr_t)q | (uintptr_t)out) & 7 || (uintptr_t)start & 3)
+        return fail(SM_E_ARG, "sm_narrow_attend: alignment (cache and work 16 bytes, rows 8)");
+    a.group = q_heads / a.s.heads; a.rows = rows; a.R = rows * a.group; a.J = (span + NCHUNK - 1) / NCHUNK;
+    if ((i64)((a.J + 3) / 4) * ((a.R + 3) / 4) > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_attend: too many rows at this span for one call");
+    const NarrowWork w = narrow_work(a.s, a.R, a.J);
+    if (work_bytes < w.bytes) return fail(SM_E_ARG, "sm_narrow_attend: the workspace is smaller than sm_narrow_work");
+    OnDevice on(buf);
+    if (!on.ok) return fail(SM_E_ARG, "sm_narrow_attend: the cache is not in a device's memory");
+    char* wk = static_cast<char*>(work);
+    a.buf = static_cast<const char*>(buf);
+    a.q = (const i64*)q; a.q_row = q_row; a.q_stream = q_stream; a.out = (i64*)out; a.o_row = out_row; a.o_stream = out_stream;
+    a.start = start; a.count = count; a.span = span; a.F = scale; a.tb = t->tb();
+    a.q8 = reinterpret_cast<signed char*>(wk + w.q8); a.eq = reinterpret_cast<int*>(wk + w.eq); a.pos = reinterpret_cast<int*>(wk + w.pos);
+    a.pm = reinterpret_cast<float*>(wk + w.pm); a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
+    a.pN = reinterpret_cast<int*>(wk + w.pN);
+    hipStream_t st = (hipStream_t)stream;
+    launch(g_kt.stages, "narrow.q", k_narrow_q, dim3((unsigned)((rows * q_heads + 3) / 4), 1, (unsigned)a.s.streams), dim3(NTHREADS), 0, st, a);
+    if (a.s.bits == 4) a.s.wide == 64 ? narrow_split<4, 1>(a, st) : a.s.wide == 128 ? narrow_split<4, 2>(a, st) : narrow_split<4, 4>(a, st);
+    else a.s.wide == 64 ? narrow_split<8, 1>(a, st) : a.s.wide == 128 ? narrow_split<8, 2>(a, st) : narrow_split<8, 4>(a, st);
+    launch(g_kt.stages, "narrow.join", k_narrow_join, dim3((unsigned)a.R, (unsigned)a.s.heads, (unsigned)a.s.streams), dim3(NTHREADS), 0, st, a);
+    HIP_TRY(hipGetLastError());
+    return SM_OK;
+}

@@ -36,6 +36,11 @@ class SmConfig(ctypes.Structure):
                 ("v64", ctypes.c_int32)]
 
 
+class Narrow(ctypes.Structure):
+    """sm_narrow of include/sm_base2.h: a cache's shape"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("streams", "heads", "dim", "ctx", "bits")]
+
+
 FLOAT_STAGES = dict(gauge=1, edge=2, arrival=4, turn=8)     # SM_FLOAT_* of include/sm_base2.h
 
 
@@ -91,6 +96,15 @@ def lib():
         L.sm_plate_product_rows_noalloc.argtypes = [vp, vp, i32, vp, vp]
         L.sm_plate_bytes.restype = i64
         L.sm_plate_bytes.argtypes = [vp]
+        nsp = ctypes.POINTER(Narrow)
+        L.sm_plate8_create.argtypes = [ctypes.POINTER(ctypes.c_int8), i32p, i64p, i32, i32, ctypes.POINTER(vp)]
+        L.sm_plate8_destroy.argtypes = [vp]
+        L.sm_plate8_product.argtypes = [vp, vp, i64, i32, vp, i64, vp, i64, vp]
+        L.sm_narrow_write.argtypes = L.sm_narrow_read.argtypes = [nsp, vp, vp, vp, i64, i64, i32, vp, vp, vp]
+        L.sm_narrow_attend.argtypes = [vp, nsp, vp, vp, i64, i64, i32, i32, i32, vp, vp, i32, vp, i64, i64, vp, i64, vp]
+        for f, args in (("sm_plate8_bytes", [vp]), ("sm_plate8_work", [vp, i32]), ("sm_narrow_bytes", [nsp]),
+                        ("sm_narrow_work", [nsp, i32, i32, i32])):
+            getattr(L, f).restype, getattr(L, f).argtypes = i64, args
         _LIB = L
     return _LIB
 
@@ -324,6 +338,92 @@ class Plate:
             self.h = None
 
     __del__ = close
+
+
+def _size(n: int) -> int:
+    """a size in bytes, or the error it stands for"""
+    check(min(n, 0))
+    return n
+
+
+class Plate8:
+    """A plate of 8-bit digits on the device: w int8 [nin][nout] (input-major, on the host), a power of two e and a bias b
+    (at 2^-16) for each column; any nin up to 131,071 and any nout (convert.py: cols8 and stream make them).
+
+    .product: out[r] = rsh(x8 . w, -(e + ex + 16)) + b for rows of int64, each row's 8-bit digits x8 and level ex formed in
+    the call.  work: a device buffer of work_bytes(rows) bytes (16 bytes' alignment) that the call uses until its kernels
+    have run: calls that may overlap have one each.  Nothing is allocated and nothing waited for."""
+
+    def __init__(self, w, e, b):
+        self.L = lib()
+        w, e, b = _np(w, np.int8), _np(e, np.int32), _np(b, np.int64)
+        if w.ndim != 2 or e.shape != w.shape[1:] or b.shape != w.shape[1:]:
+            raise ValueError(f"Plate8: w [nin][nout], e [nout], b [nout]: got {w.shape}, {e.shape}, {b.shape}")
+        self.nin, self.nout = w.shape
+        h = vp()
+        check(self.L.sm_plate8_create(w.ctypes.data_as(ctypes.POINTER(ctypes.c_int8)), e.ctypes.data_as(i32p),
+                                      b.ctypes.data_as(i64p), self.nin, self.nout, ctypes.byref(h)))
+        self.h = h
+        self.bytes = int(self.L.sm_plate8_bytes(self.h))
+
+    def work_bytes(self, rows: int) -> int:
+        return _size(self.L.sm_plate8_work(self.h, rows))
+
+    def product(self, x, rows, out, work, work_bytes, x_stride=0, out_stride=0, stream=0):
+        """x, out, work: device pointers; the strides in values (0: dense rows)"""
+        check(self.L.sm_plate8_product(self.h, x, x_stride or self.nin, rows, out, out_stride or self.nout, work, work_bytes,
+                                       stream))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.L.sm_plate8_destroy(self.h)
+            self.h = None
+
+    __del__ = close
+
+
+class NarrowCache:
+    """The shape of a cache of 4 or 8-bit digits (heads of up to 256 dimensions, a level for each head's row of k and of v)
+    and the operators on it.  The cache itself is `bytes` bytes of device memory of the caller's (16 bytes' alignment);
+    zeroed memory is an empty cache.
+
+    Every pointer is a device pointer.  start, count: int32 [streams], the first position and the number of rows of each
+    stream in this call (count 0: `rows` for every stream); rows past it, and positions that the cache (attend: span) does
+    not have, are left out and their outputs stay.  Strides are in values; 0 means dense [streams][rows][heads][dim]."""
+
+    def __init__(self, streams: int, heads: int, dim: int, ctx: int, bits: int = 4):
+        self.L = lib()
+        self.shape = Narrow(streams, heads, dim, ctx, bits)
+        self._ref = ctypes.byref(self.shape)
+        self.bytes = _size(self.L.sm_narrow_bytes(self._ref))
+        self.scale = -round(np.log2(dim) / 2 * 65536)        # the scores' usual 1 / sqrt(dim)
+
+    def _strides(self, rows, heads, row_stride, stream_stride):
+        row = row_stride or heads * self.shape.dim
+        return row, stream_stride or rows * row
+
+    def write(self, cache, k, v, rows, start, count=0, row_stride=0, stream_stride=0, stream=0):
+        """int64 rows of k and v into their positions' digits and levels"""
+        row, st = self._strides(rows, self.shape.heads, row_stride, stream_stride)
+        check(self.L.sm_narrow_write(self._ref, cache, k, v, row, st, rows, start, count, stream))
+
+    def read(self, cache, k, v, rows, start, count=0, row_stride=0, stream_stride=0, stream=0):
+        """the values that the digits of those positions stand for, into k and v"""
+        row, st = self._strides(rows, self.shape.heads, row_stride, stream_stride)
+        check(self.L.sm_narrow_read(self._ref, cache, k, v, row, st, rows, start, count, stream))
+
+    def work_bytes(self, q_heads: int, rows: int, span: int) -> int:
+        return _size(self.L.sm_narrow_work(self._ref, q_heads, rows, span))
+
+    def attend(self, t: Tables, cache, q, q_heads, rows, span, start, count, out, work, work_bytes, scale=None, q_row=0,
+               q_stream=0, out_row=0, out_stream=0, stream=0):
+        """out: each row's attention over positions 0 .. its own (written before), query head i over key head
+        i / (q_heads / heads); no row's position reaches span.  scale: log2 of the scores' scale at 2^-16 (None:
+        1 / sqrt(dim)).  work: work_bytes(q_heads, rows, span) bytes that the call uses until its kernels have run."""
+        qr, qs = self._strides(rows, q_heads, q_row, q_stream)
+        outr, outs = self._strides(rows, q_heads, out_row, out_stream)
+        check(self.L.sm_narrow_attend(t.h, self._ref, cache, q, qr, qs, q_heads, rows, span, start, count,
+                                      self.scale if scale is None else scale, out, outr, outs, work, work_bytes, stream))
 
 
 class stages:
