@@ -36,31 +36,42 @@ struct Narrow8Args {
     i64* out; i64 ldo;
 };
 
+// four values of a row from place 4 q, zeros past its end (rows stand at 8 bytes' alignment only)
+typedef i64 i64x2 __attribute__((ext_vector_type(2), aligned(8)));
+SMD void row_quad(const i64* x, int q, int nin, i64 v[4]) {
+    if (4 * q + 3 < nin) {
+        const i64x2 lo = *reinterpret_cast<const i64x2*>(x + 4 * q), hi = *reinterpret_cast<const i64x2*>(x + 4 * q + 2);
+        v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = 4 * q + i < nin ? x[4 * q + i] : 0;
+    }
+}
 // one block a row: the row's level, then its digits in the operand's order (four in a row a thread).  Rows of up to
-// 8,192 values are held in registers between the two passes, longer ones are read again.
+// 8,192 values are held in registers between the two passes, longer ones are read again.  Bound by the rows' read.  The 16
+// rows of a tile share their 128-byte lines of digits: with many rows, blocks of one die (every eighth) take one tile, so
+// that the lines fill in that die's L2.
 __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
     constexpr int HOLD = 8;
     __shared__ u64 wor[NTHREADS / 64];
-    const int r = blockIdx.x, tid = threadIdx.x, quads = a.K / 4;
+    const int b = blockIdx.x, r = gridDim.x >= 128 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
+    const int tid = threadIdx.x, quads = a.K / 4;
+    if (r >= a.rows) return;
     const i64* x = a.X + (i64)r * a.ldx;
-    auto load = [&](int q, i64 v[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = 4 * q + i < a.nin ? x[4 * q + i] : 0;
-    };
     i64 held[HOLD][4];
     u64 orr = 0;
 #pragma unroll
     for (int s = 0; s < HOLD; s++) {
         const int q = tid + s * NTHREADS;
         if (q < quads) {
-            load(q, held[s]);
+            row_quad(x, q, a.nin, held[s]);
 #pragma unroll
             for (int i = 0; i < 4; i++) orr |= mag64(held[s][i]);
         }
     }
     for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
         i64 v[4];
-        load(q, v);
+        row_quad(x, q, a.nin, v);
 #pragma unroll
         for (int i = 0; i < 4; i++) orr |= mag64(v[i]);
     }
@@ -85,16 +96,17 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
         if (tid + s * NTHREADS < quads) store(tid + s * NTHREADS, held[s]);
     for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
         i64 v[4];
-        load(q, v);
+        row_quad(x, q, a.nin, v);
         store(q, v);
     }
 }
 
 SMD v4i mfma8(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-// rsh(pile, -(e + ex + 16)) + b
+// rsh(pile, -(e + ex + 16)) + b; a pile shifted right by 32 places or more rounds to 0
 SMD i64 narrow_out(int pile, int we, int sh, i64 wb) {
     const int s = -(we + sh);
-    return wadd(s > 0 ? rsh_round(pile, min(s, 63)) : shl(pile, -s), wb);
+    if (s <= 0) return wadd(shl(pile, -s), wb);
+    return wadd(s > 31 ? 0 : (pile >> s) + ((pile >> (s - 1)) & 1), wb);
 }
 
 // RT row tiles by CT column tiles a wave, the inputs split over KW of a block's four waves and their piles added
@@ -141,6 +153,100 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
             const int row = (rt0 + t / CT) * 16 + 4 * (lane >> 4) + i;
             if (row < a.rows) a.out[(i64)row * a.ldo + col] = narrow_out(p[i], we, a.level[row], wb);
         }
+    }
+}
+
+// The product of many rows: WR x WC waves of RT x CT tiles each.  Every step of 64 inputs is a stage of (WR RT + WC CT)
+// fragments of 1 KB, loaded from memory straight into LDS in the operands' order (so neither the loads nor the operand
+// reads rearrange anything and no two lanes meet in a bank), ST - 1 stages ahead.
+typedef const __attribute__((address_space(1))) void* gas_p;
+typedef __attribute__((address_space(3))) void* las_p;
+template <int WR, int WC, int RT, int CT>
+__global__ __launch_bounds__(64 * WR * WC, 2) void k_narrow_tiles(Narrow8Args a, int tr, int tc) {
+    constexpr int W = WR * WC, AF = WR * RT, F = AF + WC * CT, LPW = F / W;
+    static_assert(F % W == 0, "every wave loads the same number of fragments");
+    __shared__ v4i s0[F * 64], s1[F * 64], s2[F * 64], s3[F * 64];
+    // consecutive blocks go to the eight dies in turn: each takes a run of tiles, eight row tiles by turns, so that the
+    // blocks that share a die's L2 share their rows and columns
+    const int per = (tr * tc + 7) / 8, l = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || l >= tr * tc) return;
+    const int grp = l / (8 * tc), gr = min(8, tr - grp * 8), in = l - grp * 8 * tc, br = grp * 8 + in % gr, bc = in / gr;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC;
+    const int kbs = a.K / 64, rts = (a.rows + 15) / 16, nt = (a.N + 15) / 16;
+    const v4i* src[LPW];
+#pragma unroll
+    for (int i = 0; i < LPW; i++) {
+        const int f = wave * LPW + i;
+        const signed char* base = f < AF ? a.lights + (i64)min(br * AF + f, rts - 1) * a.K * 16
+                                         : a.W + (i64)min(bc * WC * CT + f - AF, nt - 1) * a.K * 16;
+        src[i] = reinterpret_cast<const v4i*>(base) + lane;
+    }
+    auto fetch = [&](v4i* buf, int k) {
+        k = min(k, kbs - 1);             // (past the end: the last stage again, never read)
+#pragma unroll
+        for (int i = 0; i < LPW; i++)
+            __builtin_amdgcn_global_load_lds((gas_p)(src[i] + k * 64), (las_p)(buf + (wave * LPW + i) * 64), 16, 0, 0);
+    };
+    v4i acc[RT][CT] = {};
+    struct Operands { v4i x[RT], w[CT]; } even, odd;
+    auto read = [&](const v4i* buf, Operands& o) {
+#pragma unroll
+        for (int r = 0; r < RT; r++) o.x[r] = buf[(wr * RT + r) * 64 + lane];
+#pragma unroll
+        for (int c = 0; c < CT; c++) o.w[c] = buf[(AF + wc * CT + c) * 64 + lane];
+    };
+    // Step k's operands are in registers (read from stage k the step before); stage k + 1 is whole once every wave's loads
+    // of it have landed (all but the two stages' after it) and the waves have met, and then nobody reads stage k any more:
+    // its place takes stage k + 4.
+    auto step = [&](v4i* now, const v4i* next, const Operands& o, Operands& on, int k) {
+        __builtin_amdgcn_s_waitcnt(0x0070 | ((2 * LPW) & 15) | ((2 * LPW) >> 4) << 14);      // vmcnt(2 LPW) lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(now, k + 4);
+        read(next, on);
+        if (k < kbs) {
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int c = 0; c < CT; c++) acc[r][c] = mfma8(o.x[r], o.w[c], acc[r][c]);
+        }
+    };
+    fetch(s0, 0);
+    fetch(s1, 1);
+    fetch(s2, 2);
+    fetch(s3, 3);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | ((3 * LPW) & 15) | ((3 * LPW) >> 4) << 14);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(s0, even);
+    for (int k = 0; k < kbs; k += 4) {
+        step(s0, s1, even, odd, k);
+        step(s1, s2, odd, even, k + 1);
+        step(s2, s3, even, odd, k + 2);
+        step(s3, s0, odd, even, k + 3);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);              // no load into LDS outlives its wave
+    const int n = lane & 15, g = lane >> 4;
+    int lev[RT][4];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lev[r][i] = a.level[min((br * AF + wr * RT + r) * 16 + 4 * g + i, a.rows - 1)];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const int col = (bc * WC * CT + wc * CT + c) * 16 + n;
+        if (col >= a.N) continue;
+        const int we = a.we[col];
+        const i64 wb = a.wb[col];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = (br * AF + wr * RT + r) * 16 + 4 * g + i;
+                if (row < a.rows) a.out[(i64)row * a.ldo + col] = narrow_out(acc[r][c][i], we, lev[r][i], wb);
+            }
     }
 }
 
@@ -575,49 +681,61 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblo
         }
 }
 
-// a block a row: its chunks joined
-__global__ __launch_bounds__(NTHREADS) void k_narrow_join(NarrowAtt a) {
-    __shared__ float sm[4];
-    __shared__ int se[4];
-    __shared__ i64 sa[4];
-    __shared__ i64 sn[NTHREADS];
+// A block a row: its chunks joined.  The chunks' factors and shifts are formed once, in LDS, a batch of NT chunks at a
+// time; then NT / wide slices of chunks, a thread a dimension, eight loads in flight.
+template <int NT>
+__global__ __launch_bounds__(NT) void k_narrow_join(NarrowAtt a) {
+    __shared__ float sm[NT / 64];
+    __shared__ int se[NT / 64], sf[NT], ss[NT];
+    __shared__ i64 sa[NT / 64], sn[NT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rho = blockIdx.x, h = blockIdx.y, stream = blockIdx.z;
-    const i64 head = (i64)stream * a.s.heads + h;
+    const i64 head = (i64)stream * a.s.heads + h, slot0 = head * a.J * a.R + rho;
     const int p = a.pos[head * a.R + rho];
     if (p < 0) return;
     const int J = p / NCHUNK + 1;
     float M = -3e9f;
     int E = 0;
-    for (int j = tid; j < J; j += NTHREADS) {
-        const i64 s = (head * a.J + j) * a.R + rho;
-        M = fmaxf(M, a.pm[s]);
-        E = max(E, a.pE[s]);
+    for (int j = tid; j < J; j += NT) {
+        M = fmaxf(M, a.pm[slot0 + (i64)j * a.R]);
+        E = max(E, a.pE[slot0 + (i64)j * a.R]);
     }
     for (int o = 1; o < 64; o <<= 1) { M = fmaxf(M, __shfl_xor(M, o, 64)); E = max(E, __shfl_xor(E, o, 64)); }
     if (lane == 0) { sm[wave] = M; se[wave] = E; }
     __syncthreads();
-    for (int i = 0; i < 4; i++) { M = fmaxf(M, sm[i]); E = max(E, se[i]); }
-    auto f_of = [&](i64 s) {
-        const float d = M - a.pm[s];
-        return d < (float)a.tb.alen ? (i64)a.tb.ARR[(int)d] : 0;
-    };
-    i64 A = 0;
-    for (int j = tid; j < J; j += NTHREADS) {
-        const i64 s = (head * a.J + j) * a.R + rho;
-        A += rsh_round(a.pA[s] * f_of(s), 24);
+    for (int i = 0; i < NT / 64; i++) { M = fmaxf(M, sm[i]); E = max(E, se[i]); }
+    const int wide = a.s.wide, d = tid % wide, slice = tid / wide, slices = NT / wide;
+    i64 A = 0, N = 0;
+    for (int j0 = 0; j0 < J; j0 += NT) {
+        const int n = min(NT, J - j0);
+        __syncthreads();
+        if (tid < n) {
+            const i64 s = slot0 + (i64)(j0 + tid) * a.R;
+            const float df = M - a.pm[s];
+            const int f = df < (float)a.tb.alen ? a.tb.ARR[(int)df] : 0;
+            A += rsh_round((i64)a.pA[s] * f, 24);
+            sf[tid] = f;
+            ss[tid] = min(24 + E - a.pE[s], 63);
+        }
+        __syncthreads();
+        const int* pn = a.pN + (slot0 + (i64)j0 * a.R) * wide + d;
+        const i64 step = (i64)a.R * wide;
+        int j = slice;
+        for (; j + 7 * slices < n; j += 8 * slices) {
+            int v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = pn[(j + i * slices) * step];
+#pragma unroll
+            for (int i = 0; i < 8; i++) N += rsh_round((i64)v[i] * sf[j + i * slices], ss[j + i * slices]);
+        }
+        for (; j < n; j += slices) N += rsh_round((i64)pn[j * step] * sf[j], ss[j]);
     }
     A = wave_reduce64(A, OpAdd());
     if (lane == 0) sa[wave] = A;
-    const int wide = a.s.wide, d = tid % wide, slice = tid / wide, slices = NTHREADS / wide;
-    i64 N = 0;
-    for (int j = slice; j < J; j += slices) {
-        const i64 s = (head * a.J + j) * a.R + rho;
-        N += rsh_round(a.pN[s * wide + d] * f_of(s), min(24 + E - a.pE[s], 63));
-    }
     sn[tid] = N;
     __syncthreads();
     if (tid >= a.s.dim) return;
-    A = sa[0] + sa[1] + sa[2] + sa[3];
+    A = 0;
+    for (int i = 0; i < NT / 64; i++) A += sa[i];
     for (int i = 1; i < slices; i++) N += sn[i * wide + d];
     const int t = rho / a.group, hq = h * a.group + rho % a.group;
     a.out[stream * a.o_stream + t * a.o_row + (i64)hq * a.s.dim + d] = power(N, ((i64)E + 8) * 65536 - log2fix(A, a.tb), a.tb);
@@ -718,11 +836,19 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     a.lights = static_cast<signed char*>(work);
     a.level = reinterpret_cast<int*>(static_cast<char*>(work) + plate8_lights(p, rows));
     hipStream_t s = (hipStream_t)stream;
-    launch(g_kt.stages, "plate8.lights", k_narrow_lights, dim3(rows), dim3(NTHREADS), 0, s, a);
+    launch(g_kt.stages, "plate8.lights", k_narrow_lights, dim3((unsigned)(rows < 128 ? rows : (rows + 127) / 128 * 128)), dim3(NTHREADS), 0, s, a);
     const int nt = (a.N + 15) / 16, rts = (rows + 15) / 16;
     if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
     else if (rts == 2) launch(g_kt.stages, "plate8.rows", k_narrow_rows<2, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
-    else launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3(nt, (rts + 3) / 4), dim3(NTHREADS), 0, s, a);
+    else if (rows <= 256) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3(nt, (rts + 3) / 4), dim3(NTHREADS), 0, s, a);
+    else {
+        auto tiles = [&](auto kern, int rt, int ct, int threads) {
+            const int tr = (rts + rt - 1) / rt, tc = (nt + ct - 1) / ct;
+            launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)((tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
+        };
+        if ((i64)((rts + 15) / 16) * ((nt + 15) / 16) >= 192) tiles(k_narrow_tiles<2, 4, 8, 4>, 16, 16, 512);
+        else tiles(k_narrow_tiles<2, 2, 4, 4>, 8, 8, 256);
+    }
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
@@ -864,7 +990,9 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     launch(g_kt.stages, "narrow.q", k_narrow_q, dim3((unsigned)((rows * q_heads + 3) / 4), 1, (unsigned)a.s.streams), dim3(NTHREADS), 0, st, a);
     if (a.s.bits == 4) a.s.wide == 64 ? narrow_split<4, 1>(a, st) : a.s.wide == 128 ? narrow_split<4, 2>(a, st) : narrow_split<4, 4>(a, st);
     else a.s.wide == 64 ? narrow_split<8, 1>(a, st) : a.s.wide == 128 ? narrow_split<8, 2>(a, st) : narrow_split<8, 4>(a, st);
-    launch(g_kt.stages, "narrow.join", k_narrow_join, dim3((unsigned)a.R, (unsigned)a.s.heads, (unsigned)a.s.streams), dim3(NTHREADS), 0, st, a);
+    const dim3 rgrid((unsigned)a.R, (unsigned)a.s.heads, (unsigned)a.s.streams);
+    if (a.J > 32) launch(g_kt.stages, "narrow.join", k_narrow_join<1024>, rgrid, dim3(1024), 0, st, a);
+    else launch(g_kt.stages, "narrow.join", k_narrow_join<256>, rgrid, dim3(256), 0, st, a);
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
