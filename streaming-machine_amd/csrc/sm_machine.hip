@@ -282,6 +282,7 @@ static void free_mfma_plate(MfmaPlate& P) {
 struct sm_tables {
     int* LOG2 = nullptr; int* EXP2 = nullptr; int* PHI = nullptr; int* ARR = nullptr;
     int* GPOW = nullptr; int* HPOW = nullptr; int* PGPOW = nullptr;
+    int* ARR2 = nullptr;      // [alen + 1] 2 rsh(ARR[d], 2), a 0 at the end: the narrow attention's weights
     int alen = 0;
     i64 log768 = 0, eps40 = 0;
     int verified = 0;         // every entry equals its defining formula (checked on the device at create)
@@ -316,6 +317,11 @@ static int tables_init(sm_tables& T, const i64* phi, const i64* arr, int alen, c
     int rc;
     if ((rc = upload_table(&T.PHI, phi, 65536, 0, 65536, "phi"))) return rc;
     if ((rc = upload_table(&T.ARR, arr, alen, 0, 1 << 24, "arrival"))) return rc;
+    {
+        std::vector<i64> w(alen + 1, 0);
+        for (int d = 0; d < alen; d++) w[d] = (arr[d] + 2) >> 2 << 1;
+        if ((rc = upload_table(&T.ARR2, w.data(), w.size(), 0, 1 << 23, "arrival weights"))) return rc;
+    }
     if ((rc = upload_table(&T.LOG2, log2t, 65536, 0, 65536, "log2"))) return rc;
     if ((rc = upload_table(&T.EXP2, exp2t, 65536, 65536, 131072, "exp2"))) return rc;
     // derived tables: exact integer compositions of LOG2 and EXP2 (see Tables in sm_device.h)
@@ -360,7 +366,7 @@ static int stage_init(sm_tables& T) {
 }
 
 static void tables_free(sm_tables& T) {
-    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
+    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.ARR2); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
     hfree(T.asc); hfree(T.acm); hfree(T.aacc); hfree(T.posn);
     if (T.herr) (void)hipHostFree(T.herr);
 }

@@ -436,41 +436,51 @@ struct NarrowAtt {
     const int* start; const int* count; int span; int F;
     signed char* q8;             // [streams][heads][R][wide]
     int* eq; int* pos;           // [streams][heads][R] the digits' level; the row's position, -1 a row that is not there
-    float* pm; int* pA; int* pE; int* pN;   // [streams][heads][J][R] each chunk's m_j, A_j, E_j and (x wide) N_j
+    int* pm; int* pA; int* pE; int* pN;     // [streams][heads][J][R] each chunk's m_j, A_j, E_j and (x wide) N_j
+    const int* W2;               // the arrivals' weights 2 rsh(ARR[d], 2), 0 at alen
     Tables tb;
 };
 
-// one wave a (row, query head): q's digits
-__global__ __launch_bounds__(NTHREADS) void k_narrow_q(NarrowAtt a) {
-    const int lane = threadIdx.x & 63, stream = blockIdx.z, q_heads = a.s.heads * a.group;
-    const int i = blockIdx.x * (NTHREADS / 64) + (threadIdx.x >> 6);
-    if (i >= a.rows * q_heads) return;
-    const int t = i / q_heads, hq = i % q_heads, h = hq / a.group, rho = t * a.group + hq % a.group;
-    const i64 slot = ((i64)stream * a.s.heads + h) * a.R + rho;
+// the position of a stream's row t, -1 a row that is not there
+SMD int narrow_pos(const NarrowAtt& a, int stream, int t) {
     const i64 p = (i64)a.start[stream] + t;
-    const bool here = t < (a.count ? a.count[stream] : a.rows) && p >= 0 && p < a.span;
-    if (lane == 0) a.pos[slot] = here ? (int)p : -1;
-    i64 x[4];
+    return t < (a.count ? a.count[stream] : a.rows) && p >= 0 && p < a.span ? (int)p : -1;
+}
+// one wave: the 8-bit digits of one row's q (zeros past its dimension, and for a row that is not there) and their level
+template <int PER>
+SMD int narrow_q_row(const NarrowAtt& a, const i64* q, bool here, int lane, signed char* dst) {
+    i64 x[PER];
     u64 o = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int d = lane + 64 * j;
-        x[j] = here && d < a.s.dim ? a.q[stream * a.q_stream + t * a.q_row + (i64)hq * a.s.dim + d] : 0;
+    for (int j = 0; j < PER; j++) {
+        x[j] = here && lane + 64 * j < a.s.dim ? q[lane + 64 * j] : 0;
         o |= mag64(x[j]);
     }
     const int s16 = digit_level(wave_or_u64(o), 16);
     const i64 e = a.tb.EXP2[a.F & 0xFFFF];
     o = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < PER; j++) {
         x[j] = rsh_round(x[j], s16) * e;
         o |= mag64(x[j]);
     }
     const int s8 = digit_level(wave_or_u64(o), 8);
-    if (lane == 0) a.eq[slot] = s16 - 16 + (a.F >> 16) - 16 + s8;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (lane + 64 * j < a.s.wide) a.q8[slot * a.s.wide + lane + 64 * j] = (signed char)digit_of(x[j], s8, 8);
+    for (int j = 0; j < PER; j++) dst[lane + 64 * j] = (signed char)digit_of(x[j], s8, 8);
+    return s16 - 16 + (a.F >> 16) - 16 + s8;
+}
+
+// one wave a (row, query head): q's digits
+template <int PER>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_q(NarrowAtt a) {
+    const int lane = threadIdx.x & 63, stream = blockIdx.z, q_heads = a.s.heads * a.group;
+    const int i = blockIdx.x * (NTHREADS / 64) + (threadIdx.x >> 6);
+    if (i >= a.rows * q_heads) return;
+    const int t = i / q_heads, hq = i % q_heads, h = hq / a.group, rho = t * a.group + hq % a.group;
+    const i64 slot = ((i64)stream * a.s.heads + h) * a.R + rho;
+    const int p = narrow_pos(a, stream, t);
+    const int eq = narrow_q_row<PER>(a, a.q + stream * a.q_stream + t * a.q_row + (i64)hq * a.s.dim, p >= 0, lane, a.q8 + slot * a.s.wide);
+    if (lane == 0) { a.pos[slot] = p; a.eq[slot] = eq; }
 }
 
 // 4-bit digits of a dword as bytes of 16 times the digit (the low halves, the high halves)
@@ -490,26 +500,36 @@ SMD T row_total(T v, F op) {
     if (GR <= 8) v = op(v, __shfl_xor(v, 32, 64));
     return v;
 }
+struct IMax { SMD int operator()(int x, int y) const { return max(x, y); } };
+struct IAdd { SMD int operator()(int x, int y) const { return x + y; } };
 
-// the key operands of 16 positions from `sub`: DK x (64 dimensions)
-template <int BITS, int DK>
-SMD void key_operands(const char* keys, int sub, int lane, v4i out[DK]) {
-    const int n = lane & 15, g = lane >> 4, p = 16 * sub + n;
-    if constexpr (BITS == 8) {
+// the key digits of 16 positions from 16 `sub`, as they stand, and as DK operands (64 dimensions each)
+template <int BITS, int DK> struct KeyRaw {
+    static constexpr int U = BITS == 8 ? DK : DK / 2;
+    v4i x[U > 0 ? U : 1];
+    int2 y;
+    SMD void load(const char* keys, int sub, int n, int g) {
+        const int p = 16 * sub + n;
+        if constexpr (U > 0) {
 #pragma unroll
-        for (int u = 0; u < DK; u++) out[u] = *reinterpret_cast<const v4i*>(keys + (4 * u + g) * 1024 + p * 16);
-    } else if constexpr (DK == 1) {
-        const int2 x = *reinterpret_cast<const int2*>(keys + (g >> 1) * 1024 + p * 16 + 8 * (g & 1));
-        out[0] = v4i{nib_lo(x.x), nib_lo(x.y), nib_hi(x.x), nib_hi(x.y)};
-    } else {
+            for (int u = 0; u < U; u++) x[u] = *reinterpret_cast<const v4i*>(keys + (4 * u + g) * 1024 + p * 16);
+        } else y = *reinterpret_cast<const int2*>(keys + (g >> 1) * 1024 + p * 16 + 8 * (g & 1));
+    }
+    SMD void operands(v4i o[DK]) const {
+        if constexpr (BITS == 8) {
 #pragma unroll
-        for (int u = 0; u < DK / 2; u++) {
-            const v4i x = *reinterpret_cast<const v4i*>(keys + (4 * u + g) * 1024 + p * 16);
-            out[2 * u] = v4i{nib_lo(x[0]), nib_lo(x[1]), nib_lo(x[2]), nib_lo(x[3])};
-            out[2 * u + 1] = v4i{nib_hi(x[0]), nib_hi(x[1]), nib_hi(x[2]), nib_hi(x[3])};
+            for (int u = 0; u < DK; u++) o[u] = x[u];
+        } else if constexpr (U == 0) {
+            o[0] = v4i{nib_lo(y.x), nib_lo(y.y), nib_hi(y.x), nib_hi(y.y)};
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                o[2 * u] = v4i{nib_lo(x[u][0]), nib_lo(x[u][1]), nib_lo(x[u][2]), nib_lo(x[u][3])};
+                o[2 * u + 1] = v4i{nib_hi(x[u][0]), nib_hi(x[u][1]), nib_hi(x[u][2]), nib_hi(x[u][3])};
+            }
         }
     }
-}
+};
 // q's digits in the same order (row: the row's digits)
 template <int BITS, int DK>
 SMD void q_operands(const signed char* row, int g, v4i out[DK]) {
@@ -533,176 +553,445 @@ SMD void value_operands(v4i x, v4i out[8 / BITS]) {
         out[1] = v4i{nib_lo(x[2]), nib_lo(x[3]), nib_hi(x[2]), nib_hi(x[3])};
     }
 }
+// A score: dot 2^e rounded half up, held to 32 bits (v_cvt_rpi_i32_f32: floor(x + 1/2), saturating; dot has at most 23
+// bits, so dot 2^e is exact in float).  Compared with that function in whole numbers for every dot and every e from -60 to
+// 100: equal.
+SMD int narrow_score(int dot, int e) {
+    int s;
+    asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(s) : "v"(ldexpf((float)dot, e)));
+    return s;
+}
+// the exponent that a key's level is added to (past 40 every dot but 0 is clamped all the same)
+template <int BITS> SMD int narrow_exp(int eq) { return min(eq - 6 - (BITS == 4 ? 4 : 0), 40); }      // (4-bit operands are 16 times the digit)
+// Scores are clamped to +-2^30 where they are compared: m is clamped, and a score's distance to it is held to 0 .. far with
+// far = min(alen, m + 2^30): below 0 the score was clamped to m's 2^30, past m + 2^30 to -2^30; from alen on the arrival is 0
+#define NARROW_NONE INT_MIN         // the score of a position that a row does not see
+SMD int narrow_clamp(int m) { return min(max(m, -(1 << 30)), 1 << 30); }
+SMD int narrow_far(int m, int alen) { return (int)min((unsigned)alen, (unsigned)max(m, -(1 << 30)) + (1u << 30)); }      // (2^31 at m 2^30)
+SMD int narrow_distance(int m, int s, int far) {
+    int d;
+    asm("v_med3_i32 %0, %1, 0, %2" : "=v"(d) : "v"(__builtin_elementwise_sub_sat(m, s)), "v"(far));
+    return d;
+}
+// A weight w in 0 .. 2^22 (u shifted by the levels' distance) as three signed bytes b0 + 256 b1 + 65536 b2: w + 0x808080
+// with each byte's top bit flipped; the flip is left to the packed bytes.  u2 = 2 u, so that the shift's half is the 1 below
+SMD unsigned narrow_weight(int u2, int shift) { return (((unsigned)u2 >> shift) + 0x1010101u) >> 1; }
+// rsh(n0 + 256 n1 + 65536 n2, 8) of the byte planes' sums, the value digits of 4 bits 16 times their value
+template <int BITS> SMD int narrow_sum(int n0, int n1, int n2) {
+    const int q = n1 + (n2 << 8);
+    return BITS == 8 ? q + ((n0 + 128) >> 8) : (q + ((n0 + 2048) >> 8)) >> 4;
+}
 
-// A wave a (chunk, tile of GR rows, key head, stream).  Scores: A = q, B = keys, so a lane is a position.  With fewer than
-// 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position tiles add into
-// one accumulator: every lane then holds a score that is wanted.  Weights: byte planes through the wave's LDS, their
-// planes stacked as rows of one operand (3 GR rows in NM operands).
-template <int BITS, int DK, int GR>
-__global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblocks) {
-    constexpr int NA = GR / 4, PT = 16 / GR, NM = (3 * GR + 15) / 16, DT = 4 * DK, VU = 8 / BITS;
-    constexpr float NONE = -3e9f;
-    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][NM * 16 * 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int j = (blockIdx.x % jblocks) * (NTHREADS / 64) + wave, rt = blockIdx.x / jblocks, h = blockIdx.y, stream = blockIdx.z;
-    const i64 head = (i64)stream * a.s.heads + h;
-    // the lane's rows
-    int row[4], pos[4];
-    int er[4];
-    int phi = -1, plo = 1 << 30;
+// Few rows: a wave a chunk, a tile of GR rows (RU of every four wanted).  Scores: A = q, B = keys, so a lane is a position.
+// With fewer than 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position
+// tiles add into one accumulator: every lane then holds a score that is wanted.  Weights: byte planes through the wave's
+// LDS, their planes stacked as rows of one operand (3 GR rows in NM operands).
+template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
+    static constexpr int NA = GR / 4, PT = 16 / GR, NM = (3 * GR + 15) / 16, DT = 4 * DK, VU = 8 / BITS, WBUF = NM * 1024;
+    static constexpr int TILE_DW = DK * BITS * 2;                   // registers of a tile's keys (of its values)
+    static constexpr int AHEAD = TILE_DW <= 16 ? 4 : TILE_DW <= 32 ? 2 : 1;
+    v4i q[PT][DK];
+    int er[4], pos[4];
+    int m[4], E[4], A[4];
+    v4i C[NM][DT];
+
+    // base: the head's tiles; c0: the chunk's first position; last: the last tile that holds a position seen; whole: every
+    // row sees all 256
+    template <bool WHOLE>
+    SMD void run(const NarrowAtt& a, const char* base, int c0, int last, int lane, unsigned char* wb) {
+        const int n = lane & 15, g = lane >> 4, t0 = c0 / 64;
+        const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
+        auto tile = [&](int t) { return base + (i64)min(t0 + t, last) * tile_bytes; };
+        KeyRaw<BITS, DK> k[4][4];
+        v4i v[4][DT / VU];
+        int kl[4][NA], vl[4][NA];
+        auto load_k = [&](int t) {
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        row[r] = rt * GR + (4 * g + r) % GR;
-        const i64 slot = head * a.R + min(row[r], a.R - 1);
-        pos[r] = a.pos[slot];
-        er[r] = a.eq[slot] - 6 - (BITS == 4 ? 4 : 0);
-        phi = max(phi, pos[r]);
-        plo = min(plo, pos[r]);
+            for (int sub = 0; sub < 4; sub++) k[t][sub].load(tile(t), sub, n, g);
+        };
+        auto load_v = [&](int t) {
+#pragma unroll
+            for (int c = 0; c < DT / VU; c++) v[t][c] = *reinterpret_cast<const v4i*>(tile(t) + half + c * 1024 + lane * 16);
+        };
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const unsigned char* lev = reinterpret_cast<const unsigned char*>(tile(t) + 2 * half);
+#pragma unroll
+            for (int x = 0; x < NA; x++) {
+                kl[t][x] = lev[16 * (x * PT + 4 * g / GR) + n];
+                vl[t][x] = lev[64 + 16 * (x * PT + 4 * g / GR) + n];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < AHEAD; t++) load_k(t);
+        int sc[4][NA][RU];
+#pragma unroll
+        for (int r = 0; r < RU; r++) { m[r] = NARROW_NONE; E[r] = 0; A[r] = 0; }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if (t + AHEAD < 4) load_k(t + AHEAD);
+            else load_v(t + AHEAD - 4);
+            v4i acc[NA] = {};
+#pragma unroll
+            for (int sub = 0; sub < 4; sub++) {
+                v4i o[DK];
+                k[t][sub].operands(o);
+#pragma unroll
+                for (int u = 0; u < DK; u++) acc[sub / PT] = mfma8(q[sub % PT][u], o[u], acc[sub / PT]);
+            }
+#pragma unroll
+            for (int x = 0; x < NA; x++) {
+                const int i = c0 + 64 * t + 16 * (x * PT + 4 * g / GR) + n;
+#pragma unroll
+                for (int r = 0; r < RU; r++) {
+                    sc[t][x][r] = narrow_score(acc[x][r], er[r] + kl[t][x]);
+                    m[r] = WHOLE || i <= pos[r] ? max(m[r], sc[t][x][r]) : m[r];
+                    if (!WHOLE || r == 0) E[r] = max(E[r], WHOLE || i <= pos[r] ? vl[t][x] : 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RU; r++) {
+            m[r] = row_total<GR>(m[r], IMax());
+            // (every row sees the same levels where each sees all: the total over all lanes)
+            if (WHOLE) E[r] = r == 0 ? row_total<4>(E[0], IMax()) : E[0];
+            else E[r] = row_total<GR>(E[r], IMax());
+        }
+        int far[RU];
+#pragma unroll
+        for (int r = 0; r < RU; r++) {
+            m[r] = WHOLE || c0 <= pos[r] ? narrow_clamp(m[r]) : NARROW_NONE;
+            far[r] = narrow_far(m[r], a.tb.alen);
+        }
+#pragma unroll
+        for (int k2 = 0; k2 < NM; k2++)
+#pragma unroll
+            for (int c = 0; c < DT; c++) C[k2][c] = v4i{};
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if (t >= 1 && t + AHEAD - 1 < 4 && AHEAD < 4) load_v(t + AHEAD - 1);
+#pragma unroll
+            for (int x = 0; x < NA; x++) {
+                const int T = x * PT + 4 * g / GR, o = 16 * (n >> 2) + 4 * T + (n & 3);
+#pragma unroll
+                for (int r = 0; r < RU; r++) {
+                    int d = narrow_distance(m[r], sc[t][x][r], far[r]), sh = min(E[r] - vl[t][x], 31);
+                    if (!WHOLE) {
+                        if (c0 + 64 * t + 16 * T + n > pos[r]) d = a.tb.alen;
+                        sh = max(sh, 0);
+                    }
+                    const int u2 = a.W2[d];
+                    A[r] += u2;
+                    const unsigned b = narrow_weight(u2, sh) ^ 0x808080u;
+                    const int row0 = (4 * g + r) % GR;
+                    wb[row0 * 64 + o] = (unsigned char)b;
+                    wb[(GR + row0) * 64 + o] = (unsigned char)(b >> 8);
+                    wb[(2 * GR + row0) * 64 + o] = (unsigned char)(b >> 16);
+                }
+            }
+            v4i w[NM];
+#pragma unroll
+            for (int k2 = 0; k2 < NM; k2++) w[k2] = *reinterpret_cast<const v4i*>(wb + (16 * k2 + n) * 64 + 16 * g);
+#pragma unroll
+            for (int c = 0; c < DT / VU; c++) {
+                v4i o[VU];
+                value_operands<BITS>(v[t][c], o);
+#pragma unroll
+                for (int y = 0; y < VU; y++)
+#pragma unroll
+                    for (int k2 = 0; k2 < NM; k2++) C[k2][c * VU + y] = mfma8(w[k2], o[y], C[k2][c * VU + y]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RU; r++) A[r] = (int)((unsigned)row_total<GR>(A[r], IAdd()) >> 1);     // (2^31 at most)
     }
-    phi = max(phi, __shfl_xor(phi, 16, 64)); phi = max(phi, __shfl_xor(phi, 32, 64));
-    plo = min(plo, __shfl_xor(plo, 16, 64)); plo = min(plo, __shfl_xor(plo, 32, 64));
-    phi = __builtin_amdgcn_readfirstlane(phi);
-    plo = __builtin_amdgcn_readfirstlane(plo);
+    // N_j of dimension tile c and the lane's row r (lane groups g < GR / 4 hold the rows)
+    SMD int sum(int c, int r) const {
+        const int n0 = C[0][c][r];
+        if constexpr (GR == 16) return narrow_sum<BITS>(n0, C[1][c][r], C[2][c][r]);
+        else if constexpr (GR == 8) return narrow_sum<BITS>(n0, __shfl_xor(n0, 32, 64), C[1][c][r]);
+        else return narrow_sum<BITS>(n0, __shfl_xor(n0, 16, 64), __shfl_xor(n0, 32, 64));
+    }
+};
+
+// a block: NTHREADS / 64 chunks of one row tile, their partial sums to memory (k_narrow_join)
+template <int BITS, int DK, int GR, int RU>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblocks) {
+    using Chunk = NarrowChunk<BITS, DK, GR, RU>;
+    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
+    __shared__ __attribute__((aligned(16))) signed char qd[GR][64 * DK];
+    __shared__ int qe[GR], qp[GR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int jb = blockIdx.x % jblocks, j = jb * (NTHREADS / 64) + wave, rt = blockIdx.x / jblocks, h = blockIdx.y, stream = blockIdx.z;
+    const i64 head = (i64)stream * a.s.heads + h;
+    // the first and the last position that the tile's rows are at (a row that is not there takes no part)
+    const int ta = rt * GR / a.group, tz = min((min(rt * GR + GR, a.R) - 1) / a.group, (a.count ? a.count[stream] : a.rows) - 1);
+    const i64 s0 = a.start[stream];
+    const int plo = (int)min(s0 + ta, (i64)a.span), phi = (int)min(s0 + tz, (i64)a.span - 1);
+    if (tz < ta || phi < jb * (NTHREADS / 64) * NCHUNK) return;
+    for (int r = wave; r < min(GR, a.R - rt * GR); r += NTHREADS / 64) {
+        const int rho = rt * GR + r, t = rho / a.group, p = narrow_pos(a, stream, t);
+        const int e = narrow_q_row<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p >= 0, lane, qd[r]);
+        if (lane == 0) { qe[r] = e; qp[r] = p; }
+    }
+    __syncthreads();
     const int c0 = j * NCHUNK;
     if (j >= a.J || c0 > phi) return;
-    const bool whole = c0 + NCHUNK - 1 <= plo;
-    // q: operand row m holds row m % GR of the tile, for the position tiles t' = m / GR alone
-    v4i q[PT][DK];
-    {
-        const int m = n;
-        v4i x[DK];
-        q_operands<BITS, DK>(a.q8 + (head * a.R + min(rt * GR + m % GR, a.R - 1)) * a.s.wide, g, x);
+    Chunk c;
+    v4i x[DK];
+    q_operands<BITS, DK>(qd[min(n % GR, a.R - rt * GR - 1)], g, x);
 #pragma unroll
-        for (int t = 0; t < PT; t++)
+    for (int t = 0; t < Chunk::PT; t++)
 #pragma unroll
-            for (int u = 0; u < DK; u++) q[t][u] = m / GR == t ? x[u] : v4i{};
+        for (int u = 0; u < DK; u++) c.q[t][u] = n / GR == t ? x[u] : v4i{};
+#pragma unroll
+    for (int r = 0; r < RU; r++) {
+        const int row = min((4 * g + r) % GR, a.R - rt * GR - 1);
+        c.er[r] = narrow_exp<BITS>(qe[row]);
+        c.pos[r] = qp[row];
     }
-    const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
-    const char* base = a.buf + head * a.s.tiles * tile_bytes;
-    const int last_tile = phi / 64;
-    float sc[4][GR];
-    int vl[4][NA];
-    float mr[4];
-    int Er[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) { mr[r] = NONE; Er[r] = 0; }
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const char* tp = base + (i64)min(4 * j + t, last_tile) * tile_bytes;
-        const unsigned char* lev = reinterpret_cast<const unsigned char*>(tp + 2 * half);
-        v4i acc[NA] = {};
-#pragma unroll
-        for (int sub = 0; sub < 4; sub++) {
-            v4i k[DK];
-            key_operands<BITS, DK>(tp, sub, lane, k);
-#pragma unroll
-            for (int u = 0; u < DK; u++) acc[sub / PT] = mfma8(q[sub % PT][u], k[u], acc[sub / PT]);
-        }
-#pragma unroll
-        for (int x = 0; x < NA; x++) {
-            const int at = 16 * (x * PT + 4 * g / GR) + n, i = c0 + 64 * t + at;
-            const int kl = lev[at];
-            vl[t][x] = lev[64 + at];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                // dot 2^-s + 1/2 is exact in float: dot has at most 23 bits, and where s <= 0 no half is needed
-                const float v = floorf(ldexpf((float)acc[x][r], er[r] + kl) + 0.5f);
-                float w = fminf(fmaxf(v, -1073741824.f), 1073741824.f);
-                if (!whole && i > pos[r]) w = NONE;
-                sc[t][4 * x + r] = w;
-                mr[r] = fmaxf(mr[r], w);
-                Er[r] = max(Er[r], whole || i <= pos[r] ? vl[t][x] : 0);
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        mr[r] = row_total<GR>(mr[r], [](float x, float y) { return fmaxf(x, y); });
-        Er[r] = row_total<GR>(Er[r], [](int x, int y) { return max(x, y); });
-    }
-    v4i C[NM][DT] = {};
-    int A[4] = {};
-    unsigned char* wb = wbuf[wave];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const char* vp = base + (i64)min(4 * j + t, last_tile) * tile_bytes + half;
-        v4i v[DT / VU];
-#pragma unroll
-        for (int c = 0; c < DT / VU; c++) v[c] = *reinterpret_cast<const v4i*>(vp + c * 1024 + lane * 16);
-#pragma unroll
-        for (int x = 0; x < NA; x++) {
-            const int T = x * PT + 4 * g / GR;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float d = fminf(mr[r] - sc[t][4 * x + r], (float)a.tb.alen);
-                const int i = (int)d;
-                const int u = i < a.tb.alen ? (a.tb.ARR[i] + 2) >> 2 : 0;
-                A[r] += u;
-                const int w = (((u << 1) >> min(Er[r] - vl[t][x], 31)) + 1) >> 1;
-                const unsigned b = ((unsigned)w + 0x808080u) ^ 0x808080u;
-                const int row0 = (4 * g + r) % GR, o = 16 * (n >> 2) + 4 * T + (n & 3);
-                wb[row0 * 64 + o] = (unsigned char)b;
-                wb[(GR + row0) * 64 + o] = (unsigned char)(b >> 8);
-                wb[(2 * GR + row0) * 64 + o] = (unsigned char)(b >> 16);
-            }
-        }
-        v4i w[NM];
-#pragma unroll
-        for (int k = 0; k < NM; k++) w[k] = *reinterpret_cast<const v4i*>(wb + (16 * k + n) * 64 + 16 * g);
-#pragma unroll
-        for (int c = 0; c < DT / VU; c++) {
-            v4i o[VU];
-            value_operands<BITS>(v[c], o);
-#pragma unroll
-            for (int y = 0; y < VU; y++)
-#pragma unroll
-                for (int k = 0; k < NM; k++) C[k][c * VU + y] = mfma8(w[k], o[y], C[k][c * VU + y]);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) A[r] = row_total<GR>(A[r], [](int x, int y) { return x + y; });
-    const i64 slot0 = (head * a.J + j) * a.R;
+    const char* base = a.buf + head * a.s.tiles * narrow_tile(a.s);
+    if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave]);
+    else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave]);
+    const i64 slot0 = (head * a.J + j) * a.R + rt * GR;
+    const int rows = a.R - rt * GR;
     if (n == 0 && 4 * g < GR)
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (row[r] < a.R) { a.pm[slot0 + row[r]] = mr[r]; a.pA[slot0 + row[r]] = A[r]; a.pE[slot0 + row[r]] = Er[r]; }
+        for (int r = 0; r < RU; r++)
+            if (4 * g + r < rows) { a.pm[slot0 + 4 * g + r] = c.m[r]; a.pA[slot0 + 4 * g + r] = c.A[r]; a.pE[slot0 + 4 * g + r] = c.E[r]; }
 #pragma unroll
-    for (int c = 0; c < DT; c++)
+    for (int d = 0; d < Chunk::DT; d++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            int n0, n1, n2;
-            if constexpr (GR == 16) { n0 = C[0][c][r]; n1 = C[1][c][r]; n2 = C[2][c][r]; }
-            else if constexpr (GR == 8) { n0 = C[0][c][r]; n1 = __shfl_xor(n0, 32, 64); n2 = C[1][c][r]; }
-            else { n0 = C[0][c][r]; n1 = __shfl_xor(n0, 16, 64); n2 = __shfl_xor(n0, 32, 64); }
-            // rsh(n0 + 256 n1 + 65536 n2, 8), the digits of 4 bits 16 times their value
-            const int q8 = n1 + (n2 << 8);
-            const int N = BITS == 8 ? q8 + ((n0 + 128) >> 8) : (q8 + ((n0 + 2048) >> 8)) >> 4;
-            if (4 * g < GR && row[r] < a.R) a.pN[(slot0 + row[r]) * a.s.wide + 16 * c + n] = N;
+        for (int r = 0; r < RU; r++) {
+            const int N = c.sum(d, r);
+            if (4 * g < GR && 4 * g + r < rows) a.pN[(slot0 + 4 * g + r) * a.s.wide + 16 * d + n] = N;
         }
+}
+
+// Many rows: a block 16 rows and all the positions that they see, its four waves every fourth chunk.  Scores: A = keys,
+// B = q, so that a lane holds one row's scores of 16 positions a tile, and exactly the ones, in the order, that its bytes of a
+// weight operand are (the values' layout): nothing moves between lanes.  A first pass over the keys finds each chunk's m_j
+// and E_j (kept in memory) and the row's M and E; the second adds each chunk's N_j f_j in registers, and the waves' sums are
+// added at the end.  Bound by the vector arithmetic of a score, so the arrivals' weights stand in LDS.
+#define SWEEP_ARR 17919            // entries of the arrival that fit (base2_convert.py:50-53 gives 17,745)
+#define SWEEP_WAVES 4
+template <int BITS, int DK>
+__global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sweep(NarrowAtt a) {
+    constexpr int DT = 4 * DK, VU = 8 / BITS, NW = SWEEP_WAVES;
+    __shared__ __attribute__((aligned(16))) int tab[SWEEP_ARR + 1];
+    __shared__ int wm[NW][16], we[NW][16];
+    __shared__ i64 wA[NW][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int h = blockIdx.y, stream = blockIdx.z;
+    const i64 head = (i64)stream * a.s.heads + h;
+    // the last rows, which see most, first
+    const int rt = (int)(gridDim.x - 1 - blockIdx.x);
+    const int rho = min(rt * 16 + n, a.R - 1), pos = a.pos[head * a.R + rho], er = narrow_exp<BITS>(a.eq[head * a.R + rho]);
+    int phi = pos, plo = pos;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) { phi = max(phi, __shfl_xor(phi, o, 64)); plo = min(plo, __shfl_xor(plo, o, 64)); }
+    phi = __builtin_amdgcn_readfirstlane(phi);
+    plo = __builtin_amdgcn_readfirstlane(plo);
+    if (phi < 0) return;                                             // (the same in every wave)
+    for (int i = threadIdx.x; i <= a.tb.alen; i += 64 * NW) tab[i] = a.W2[i];
+    v4i q[DK];
+    q_operands<BITS, DK>(a.q8 + (head * a.R + rho) * a.s.wide, g, q);
+    const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
+    const char* base = a.buf + head * a.s.tiles * tile_bytes;
+    const int last = phi / 64;
+    int* pm = a.pm + head * a.J * a.R + rho;
+    int* pE = a.pE + head * a.J * a.R + rho;
+    auto max_g = [](int v) {
+        v = max(v, __shfl_xor(v, 16, 64));
+        return max(v, __shfl_xor(v, 32, 64));
+    };
+    // a tile's keys and levels, and its values; each register takes the next tile's as soon as it has been used
+    KeyRaw<BITS, DK> k[4];
+    int kl[4], vl[4];
+    v4i v[DT / VU];
+    auto load_sub = [&](int T, int sub) {
+        const char* tp = base + (i64)T * tile_bytes;
+        k[sub].load(tp, sub, n, g);
+        kl[sub] = reinterpret_cast<const int*>(tp + 2 * half)[4 * sub + g];
+        vl[sub] = reinterpret_cast<const int*>(tp + 2 * half)[16 + 4 * sub + g];
+    };
+    auto load_v = [&](int T, int c) { v[c] = *reinterpret_cast<const v4i*>(base + (i64)T * tile_bytes + half + c * 1024 + lane * 16); };
+    auto after = [](int T) { return (T & 3) == 3 ? T + 4 * NW - 3 : T + 1; };
+    // dots of the 16 positions of a sub-tile with the lane's row, positions 4 g .. 4 g + 3 of it
+    auto dots = [&](int sub) {
+        v4i o[DK], acc = {};
+        k[sub].operands(o);
+#pragma unroll
+        for (int u = 0; u < DK; u++) acc = mfma8(o[u], q[u], acc);
+        return acc;
+    };
+    auto byte = [](int x, int r) { return (int)((unsigned)x >> 8 * r & 255u); };
+    int M = NARROW_NONE, E = 0;
+    {
+        float m = -INFINITY;
+        int e = 0;
+        int T = 4 * wave;
+#pragma unroll
+        for (int sub = 0; sub < 4; sub++) load_sub(min(T, last), sub);
+        while (T <= last) {
+            const int Tn = min(after(T), last);
+            // (rounding and clamping keep the order: done once, on the largest)
+            auto look = [&](auto whole) {
+#pragma unroll
+                for (int sub = 0; sub < 4; sub++) {
+                    const v4i acc = dots(sub);
+                    const int l = kl[sub], lv = vl[sub];
+                    load_sub(Tn, sub);
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (decltype(whole)::value || 64 * T + 16 * sub + 4 * g + r <= pos) {
+                            m = fmaxf(m, ldexpf((float)acc[r], er + byte(l, r)));
+                            e = max(e, byte(lv, r));
+                        }
+                }
+            };
+            if (64 * T + 63 <= plo) look(std::true_type());
+            else look(std::false_type());
+            if ((T & 3) == 3 || T == last) {
+                const int j = T >> 2;
+                int mi;
+                asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(mi) : "v"(m));
+                mi = max_g(j * NCHUNK + 4 * g <= pos ? narrow_clamp(mi) : NARROW_NONE);
+                e = max_g(e);
+                if (g == 0) { pm[(i64)j * a.R] = mi; pE[(i64)j * a.R] = e; }
+                M = max(M, mi);
+                E = max(E, e);
+                m = -INFINITY;
+                e = 0;
+            }
+            T = after(T);
+        }
+    }
+    if (g == 0) { wm[wave][n] = M; we[wave][n] = E; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) { M = max(M, wm[w][n]); E = max(E, we[w][n]); }
+    i64 N[DT][4] = {}, A = 0;
+    int have = -1;                                                   // the tile that is loaded
+    for (int j = wave; 4 * j <= last; j += NW) {
+        // (this wave's own stores, read by the lanes that made them)
+        const int m = __shfl(pm[(i64)j * a.R], n, 64), e = __shfl(pE[(i64)j * a.R], n, 64);
+        const unsigned df = (unsigned)M - (unsigned)m;
+        const int f = m != NARROW_NONE && df < (unsigned)a.tb.alen ? a.tb.ARR[df] : 0;
+        if (!__any(f)) continue;                                     // its sums would be multiplied by 0
+        const int far = narrow_far(m, a.tb.alen), tz = min(4 * j + 3, last);
+        v4i C[3][DT] = {};
+        unsigned Aj = 0;
+        if (have != 4 * j) {
+#pragma unroll
+            for (int sub = 0; sub < 4; sub++) load_sub(4 * j, sub);
+#pragma unroll
+            for (int c = 0; c < DT / VU; c++) load_v(4 * j, c);
+        }
+        for (int T = 4 * j; T <= tz; T++) {
+            v4i P[3];
+            have = T < tz ? T + 1 : min(4 * (j + NW), last);
+            auto weigh = [&](auto whole) {
+#pragma unroll
+                for (int sub = 0; sub < 4; sub++) {
+                    const v4i acc = dots(sub);
+                    const int l = kl[sub], lv = vl[sub];
+                    load_sub(have, sub);
+                    unsigned x[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        int d = narrow_distance(m, narrow_score(acc[r], er + byte(l, r)), far), sh = min(e - byte(lv, r), 31);
+                        if (!decltype(whole)::value) {
+                            if (64 * T + 16 * sub + 4 * g + r > pos) d = a.tb.alen;
+                            sh = max(sh, 0);
+                        }
+                        const int u2 = tab[d];
+                        Aj += u2;
+                        x[r] = narrow_weight(u2, sh);
+                    }
+                    const unsigned p01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), p23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+                    P[0][sub] = (int)(__builtin_amdgcn_perm(p23, p01, 0x05040100u) ^ 0x80808080u);
+                    P[1][sub] = (int)(__builtin_amdgcn_perm(p23, p01, 0x07060302u) ^ 0x80808080u);
+                    P[2][sub] = (int)((__builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u) | __builtin_amdgcn_perm(x[3], x[2], 0x06020c0cu)) ^ 0x80808080u);
+                }
+            };
+            if (64 * T + 63 <= plo) weigh(std::true_type());
+            else weigh(std::false_type());
+#pragma unroll
+            for (int c = 0; c < DT / VU; c++) {
+                v4i o[VU];
+                value_operands<BITS>(v[c], o);
+                load_v(have, c);
+#pragma unroll
+                for (int y = 0; y < VU; y++)
+#pragma unroll
+                    for (int p = 0; p < 3; p++) C[p][c * VU + y] = mfma8(o[y], P[p], C[p][c * VU + y]);
+            }
+        }
+        Aj += __shfl_xor(Aj, 16, 64);
+        Aj += __shfl_xor(Aj, 32, 64);
+        A += rsh_round((i64)(Aj >> 1) * f, 24);                      // (Aj 2^31 at most)
+        const int sh = min(24 + E - e, 63);
+#pragma unroll
+        for (int c = 0; c < DT; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) N[c][r] += rsh_round((i64)narrow_sum<BITS>(C[0][c][r], C[1][c][r], C[2][c][r]) * f, sh);
+    }
+    // the waves' sums through the table's place, half of a wave's a time where they are many; wave w finishes every fourth
+    // dimension tile
+    __syncthreads();
+    if (g == 0) wA[wave][n] = A;
+    i64* part = reinterpret_cast<i64*>(tab);                         // [NW][DT / HALVES][4][64]
+    constexpr int HALVES = DK == 4 ? 2 : 1, DH = DT / HALVES;
+    static_assert(NW * DH * 4 * 64 * 8 <= sizeof(tab), "the waves' sums fit the table's place");
+    const int tt = rho / a.group, hq = h * a.group + rho % a.group;
+    i64* o = a.out + stream * a.o_stream + tt * a.o_row + (i64)hq * a.s.dim;
+#pragma unroll
+    for (int hf = 0; hf < HALVES; hf++) {
+#pragma unroll
+        for (int c = 0; c < DH; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) part[((wave * DH + c) * 4 + r) * 64 + lane] = N[hf * DH + c][r];
+        __syncthreads();
+        if (hf == 0) {
+            A = 0;
+            for (int w = 0; w < NW; w++) A += wA[w][n];
+        }
+        const i64 F = ((i64)E + 8) * 65536 - log2fix(A, a.tb);
+        if (pos >= 0 && rt * 16 + n < a.R)
+            for (int c = wave; c < DH; c += NW)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    i64 s = 0;
+#pragma unroll
+                    for (int w = 0; w < NW; w++) s += part[((w * DH + c) * 4 + r) * 64 + lane];
+                    const int d = 16 * (hf * DH + c) + 4 * g + r;
+                    if (d < a.s.dim) o[d] = power(s, F, a.tb);
+                }
+        __syncthreads();
+    }
 }
 
 // A block a row: its chunks joined.  The chunks' factors and shifts are formed once, in LDS, a batch of NT chunks at a
 // time; then NT / wide slices of chunks, a thread a dimension, eight loads in flight.
 template <int NT>
 __global__ __launch_bounds__(NT) void k_narrow_join(NarrowAtt a) {
-    __shared__ float sm[NT / 64];
-    __shared__ int se[NT / 64], sf[NT], ss[NT];
+    __shared__ int sm[NT / 64], se[NT / 64], sf[NT], ss[NT];
     __shared__ i64 sa[NT / 64], sn[NT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rho = blockIdx.x, h = blockIdx.y, stream = blockIdx.z;
     const i64 head = (i64)stream * a.s.heads + h, slot0 = head * a.J * a.R + rho;
-    const int p = a.pos[head * a.R + rho];
+    const int p = narrow_pos(a, stream, rho / a.group);
     if (p < 0) return;
     const int J = p / NCHUNK + 1;
-    float M = -3e9f;
-    int E = 0;
+    int M = NARROW_NONE, E = 0;
     for (int j = tid; j < J; j += NT) {
-        M = fmaxf(M, a.pm[slot0 + (i64)j * a.R]);
+        M = max(M, a.pm[slot0 + (i64)j * a.R]);
         E = max(E, a.pE[slot0 + (i64)j * a.R]);
     }
-    for (int o = 1; o < 64; o <<= 1) { M = fmaxf(M, __shfl_xor(M, o, 64)); E = max(E, __shfl_xor(E, o, 64)); }
+    for (int o = 1; o < 64; o <<= 1) { M = max(M, __shfl_xor(M, o, 64)); E = max(E, __shfl_xor(E, o, 64)); }
     if (lane == 0) { sm[wave] = M; se[wave] = E; }
     __syncthreads();
-    for (int i = 0; i < NT / 64; i++) { M = fmaxf(M, sm[i]); E = max(E, se[i]); }
+    for (int i = 0; i < NT / 64; i++) { M = max(M, sm[i]); E = max(E, se[i]); }
     const int wide = a.s.wide, d = tid % wide, slice = tid / wide, slices = NT / wide;
     i64 A = 0, N = 0;
     for (int j0 = 0; j0 < J; j0 += NT) {
@@ -710,8 +999,8 @@ __global__ __launch_bounds__(NT) void k_narrow_join(NarrowAtt a) {
         __syncthreads();
         if (tid < n) {
             const i64 s = slot0 + (i64)(j0 + tid) * a.R;
-            const float df = M - a.pm[s];
-            const int f = df < (float)a.tb.alen ? a.tb.ARR[(int)df] : 0;
+            const unsigned df = (unsigned)M - (unsigned)a.pm[s];
+            const int f = df < (unsigned)a.tb.alen ? a.tb.ARR[df] : 0;
             A += rsh_round((i64)a.pA[s] * f, 24);
             sf[tid] = f;
             ss[tid] = min(24 + E - a.pE[s], 63);
@@ -920,19 +1209,19 @@ extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, i
     return SM_OK;
 }
 
-// ---- the attention's workspace: q's digits, the rows' levels and positions, the chunks' partial sums
-struct NarrowWork { i64 q8, eq, pos, pm, pA, pE, pN, bytes; };
+// ---- the attention's workspace: the chunks' partial sums, and with many rows q's digits, the rows' levels and positions
+struct NarrowWork { bool sweep; i64 q8, eq, pos, pm, pA, pE, pN, bytes; };
 static NarrowWork narrow_work(const NarrowShape& s, int R, int J) {
     const i64 n = (i64)s.streams * s.heads * R;
     NarrowWork w{};
-    w.q8 = 0;
-    w.eq = up256(n * s.wide);
+    w.sweep = R > 16 && (i64)s.streams * s.heads * ((R + 15) / 16) >= 256;
+    w.pm = 0;
+    w.pE = up256(n * J * 4);
+    w.pA = w.q8 = w.pE + up256(n * J * 4);
+    w.pN = w.pA + up256(n * J * 4);
+    w.eq = w.q8 + up256(n * s.wide);
     w.pos = w.eq + up256(n * 4);
-    w.pm = w.pos + up256(n * 4);
-    w.pA = w.pm + up256(n * J * 4);
-    w.pE = w.pA + up256(n * J * 4);
-    w.pN = w.pE + up256(n * J * 4);
-    w.bytes = w.pN + n * J * s.wide * 4;
+    w.bytes = w.sweep ? w.pos + n * 4 : w.pN + n * J * s.wide * 4;
     return w;
 }
 static int narrow_att_args(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span, NarrowShape& s, const char* who) {
@@ -952,12 +1241,23 @@ extern "C" int64_t sm_narrow_work(const sm_narrow* c, int32_t q_heads, int32_t r
 }
 
 template <int BITS, int DK>
-static void narrow_split(const NarrowAtt& a, hipStream_t st) {
-    const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, jb = (a.J + 3) / 4;
-    const dim3 grid((unsigned)(jb * ((a.R + gr - 1) / gr)), (unsigned)a.s.heads, (unsigned)a.s.streams);
-    if (gr == 4) launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 4>, grid, dim3(NTHREADS), 0, st, a, jb);
-    else if (gr == 8) launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 8>, grid, dim3(NTHREADS), 0, st, a, jb);
-    else launch(g_kt.stages, "narrow.attend", k_narrow_split<BITS, DK, 16>, grid, dim3(NTHREADS), 0, st, a, jb);
+static void narrow_attend(const NarrowAtt& a, bool sweep, hipStream_t st) {
+    const unsigned heads = (unsigned)a.s.heads, streams = (unsigned)a.s.streams;
+    if (sweep) {
+        launch(g_kt.stages, "narrow.q", k_narrow_q<DK>, dim3((unsigned)((a.R * a.s.heads + 3) / 4), 1, streams), dim3(NTHREADS), 0, st, a);
+        launch(g_kt.stages, "narrow.sweep", k_narrow_sweep<BITS, DK>, dim3((unsigned)((a.R + 15) / 16), heads, streams), dim3(64 * SWEEP_WAVES), 0, st, a);
+        return;
+    }
+    const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, jb = (a.J + NTHREADS / 64 - 1) / (NTHREADS / 64);
+    const dim3 grid((unsigned)(jb * ((a.R + gr - 1) / gr)), heads, streams);
+    auto split = [&](auto kern) { launch(g_kt.stages, "narrow.split", kern, grid, dim3(NTHREADS), 0, st, a, jb); };
+    if (a.R == 1) split(k_narrow_split<BITS, DK, 4, 1>);
+    else if (gr == 4) split(k_narrow_split<BITS, DK, 4, 4>);
+    else if (gr == 8) split(k_narrow_split<BITS, DK, 8, 4>);
+    else split(k_narrow_split<BITS, DK, 16, 4>);
+    const dim3 rgrid((unsigned)a.R, heads, streams);
+    if (a.J > 32) launch(g_kt.stages, "narrow.join", k_narrow_join<1024>, rgrid, dim3(1024), 0, st, a);
+    else launch(g_kt.stages, "narrow.join", k_narrow_join<256>, rgrid, dim3(256), 0, st, a);
 }
 
 extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const void* buf, const int64_t* q, int64_t q_row, int64_t q_stream,
@@ -977,6 +1277,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     if ((i64)((a.J + 3) / 4) * ((a.R + 3) / 4) > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_attend: too many rows at this span for one call");
     const NarrowWork w = narrow_work(a.s, a.R, a.J);
     if (work_bytes < w.bytes) return fail(SM_E_ARG, "sm_narrow_attend: the workspace is smaller than sm_narrow_work");
+    if (t->alen > SWEEP_ARR) return fail(SM_E_ARG, "sm_narrow_attend: the tables' arrival has more entries than the kernels hold");
     OnDevice on(buf);
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_attend: the cache is not in a device's memory");
     char* wk = static_cast<char*>(work);
@@ -984,15 +1285,11 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     a.q = (const i64*)q; a.q_row = q_row; a.q_stream = q_stream; a.out = (i64*)out; a.o_row = out_row; a.o_stream = out_stream;
     a.start = start; a.count = count; a.span = span; a.F = scale; a.tb = t->tb();
     a.q8 = reinterpret_cast<signed char*>(wk + w.q8); a.eq = reinterpret_cast<int*>(wk + w.eq); a.pos = reinterpret_cast<int*>(wk + w.pos);
-    a.pm = reinterpret_cast<float*>(wk + w.pm); a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
+    a.pm = reinterpret_cast<int*>(wk + w.pm); a.W2 = t->ARR2; a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
     a.pN = reinterpret_cast<int*>(wk + w.pN);
     hipStream_t st = (hipStream_t)stream;
-    launch(g_kt.stages, "narrow.q", k_narrow_q, dim3((unsigned)((rows * q_heads + 3) / 4), 1, (unsigned)a.s.streams), dim3(NTHREADS), 0, st, a);
-    if (a.s.bits == 4) a.s.wide == 64 ? narrow_split<4, 1>(a, st) : a.s.wide == 128 ? narrow_split<4, 2>(a, st) : narrow_split<4, 4>(a, st);
-    else a.s.wide == 64 ? narrow_split<8, 1>(a, st) : a.s.wide == 128 ? narrow_split<8, 2>(a, st) : narrow_split<8, 4>(a, st);
-    const dim3 rgrid((unsigned)a.R, (unsigned)a.s.heads, (unsigned)a.s.streams);
-    if (a.J > 32) launch(g_kt.stages, "narrow.join", k_narrow_join<1024>, rgrid, dim3(1024), 0, st, a);
-    else launch(g_kt.stages, "narrow.join", k_narrow_join<256>, rgrid, dim3(256), 0, st, a);
+    if (a.s.bits == 4) a.s.wide == 64 ? narrow_attend<4, 1>(a, w.sweep, st) : a.s.wide == 128 ? narrow_attend<4, 2>(a, w.sweep, st) : narrow_attend<4, 4>(a, w.sweep, st);
+    else a.s.wide == 64 ? narrow_attend<8, 1>(a, w.sweep, st) : a.s.wide == 128 ? narrow_attend<8, 2>(a, w.sweep, st) : narrow_attend<8, 4>(a, w.sweep, st);
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
