@@ -590,7 +590,7 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
     static constexpr int NA = GR / 4, PT = 16 / GR, NM = (3 * GR + 15) / 16, DT = 4 * DK, VU = 8 / BITS, WBUF = NM * 1024;
     static constexpr int TILE_DW = DK * BITS * 2;                   // registers of a tile's keys (of its values)
     static constexpr int AHEAD = TILE_DW <= 16 ? 4 : TILE_DW <= 32 ? 2 : 1;
-    v4i q[PT][DK];
+    v4i q[DK];
     int er[4], pos[4];
     int m[4], E[4], A[4];
     v4i C[NM][DT];
@@ -637,7 +637,7 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
                 v4i o[DK];
                 k[t][sub].operands(o);
 #pragma unroll
-                for (int u = 0; u < DK; u++) acc[sub / PT] = mfma8(q[sub % PT][u], o[u], acc[sub / PT]);
+                for (int u = 0; u < DK; u++) acc[sub / PT] = mfma8(n / GR == sub % PT ? q[u] : v4i{}, o[u], acc[sub / PT]);
             }
 #pragma unroll
             for (int x = 0; x < NA; x++) {
@@ -714,47 +714,61 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
     }
 };
 
-// a block: NTHREADS / 64 chunks of one row tile, their partial sums to memory (k_narrow_join)
-template <int BITS, int DK, int GR, int RU>
-__global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblocks) {
-    using Chunk = NarrowChunk<BITS, DK, GR, RU>;
-    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
-    __shared__ __attribute__((aligned(16))) signed char qd[GR][64 * DK];
-    __shared__ int qe[GR], qp[GR];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int jb = blockIdx.x % jblocks, j = jb * (NTHREADS / 64) + wave, rt = blockIdx.x / jblocks, h = blockIdx.y, stream = blockIdx.z;
-    const i64 head = (i64)stream * a.s.heads + h;
-    // the first and the last position that the tile's rows are at (a row that is not there takes no part)
-    const int ta = rt * GR / a.group, tz = min((min(rt * GR + GR, a.R) - 1) / a.group, (a.count ? a.count[stream] : a.rows) - 1);
+// What the blocks of few rows begin with: the positions of the tile's first and last row (a row that is not there takes no
+// part), and the rows' digits, levels and positions in LDS
+template <int DK, int GR> struct NarrowFew {
+    signed char qd[GR][64 * DK];
+    int qe[GR], qp[GR];
+};
+SMD bool narrow_reach(const NarrowAtt& a, int stream, int first, int end, int& plo, int& phi) {
+    const int ta = first / a.group, tz = min((end - 1) / a.group, (a.count ? a.count[stream] : a.rows) - 1);
     const i64 s0 = a.start[stream];
-    const int plo = (int)min(s0 + ta, (i64)a.span), phi = (int)min(s0 + tz, (i64)a.span - 1);
-    if (tz < ta || phi < jb * (NTHREADS / 64) * NCHUNK) return;
+    plo = (int)min(s0 + ta, (i64)a.span);
+    phi = (int)min(s0 + tz, (i64)a.span - 1);
+    return tz >= ta && phi >= 0;
+}
+template <int DK, int GR>
+SMD void narrow_few(const NarrowAtt& a, int stream, int h, int rt, int lane, int wave, NarrowFew<DK, GR>& f) {
     for (int r = wave; r < min(GR, a.R - rt * GR); r += NTHREADS / 64) {
         const int rho = rt * GR + r, t = rho / a.group, p = narrow_pos(a, stream, t);
-        const int e = narrow_q_row<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p >= 0, lane, qd[r]);
-        if (lane == 0) { qe[r] = e; qp[r] = p; }
+        const int e = narrow_q_row<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p >= 0, lane, f.qd[r]);
+        if (lane == 0) { f.qe[r] = e; f.qp[r] = p; }
     }
     __syncthreads();
-    const int c0 = j * NCHUNK;
-    if (j >= a.J || c0 > phi) return;
-    Chunk c;
-    v4i x[DK];
-    q_operands<BITS, DK>(qd[min(n % GR, a.R - rt * GR - 1)], g, x);
-#pragma unroll
-    for (int t = 0; t < Chunk::PT; t++)
-#pragma unroll
-        for (int u = 0; u < DK; u++) c.q[t][u] = n / GR == t ? x[u] : v4i{};
+}
+template <int BITS, int DK, int GR, int RU>
+SMD void narrow_ready(NarrowChunk<BITS, DK, GR, RU>& c, const NarrowFew<DK, GR>& f, int rows, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+    q_operands<BITS, DK>(f.qd[min(n % GR, rows - 1)], g, c.q);
 #pragma unroll
     for (int r = 0; r < RU; r++) {
-        const int row = min((4 * g + r) % GR, a.R - rt * GR - 1);
-        c.er[r] = narrow_exp<BITS>(qe[row]);
-        c.pos[r] = qp[row];
+        const int row = min((4 * g + r) % GR, rows - 1);
+        c.er[r] = narrow_exp<BITS>(f.qe[row]);
+        c.pos[r] = f.qp[row];
     }
+}
+
+// a block: NTHREADS / 64 chunks of one row tile, their partial sums to memory (k_narrow_join)
+template <int BITS, int DK, int GR, int RU>
+__global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow_split(NarrowAtt a, int jblocks) {
+    using Chunk = NarrowChunk<BITS, DK, GR, RU>;
+    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
+    __shared__ __attribute__((aligned(16))) NarrowFew<DK, GR> few;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int rt = blockIdx.x / jblocks, h = blockIdx.y, stream = blockIdx.z, rows = a.R - rt * GR;
+    // blocks go to the eight dies in turn, and a stream's late chunks may be empty: the chunks rotate with head and stream
+    const int jb = (int)((blockIdx.x + blockIdx.y + blockIdx.z) % jblocks), j = jb * (NTHREADS / 64) + wave, c0 = j * NCHUNK;
+    const i64 head = (i64)stream * a.s.heads + h;
+    int plo, phi;
+    if (!narrow_reach(a, stream, rt * GR, min(rt * GR + GR, a.R), plo, phi) || phi < jb * (NTHREADS / 64) * NCHUNK) return;
+    narrow_few<DK, GR>(a, stream, h, rt, lane, wave, few);
+    if (j >= a.J || c0 > phi) return;
+    Chunk c;
+    narrow_ready(c, few, rows, lane);
     const char* base = a.buf + head * a.s.tiles * narrow_tile(a.s);
     if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave]);
     else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave]);
     const i64 slot0 = (head * a.J + j) * a.R + rt * GR;
-    const int rows = a.R - rt * GR;
     if (n == 0 && 4 * g < GR)
 #pragma unroll
         for (int r = 0; r < RU; r++)
@@ -766,6 +780,58 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_split(NarrowAtt a, int jblo
             const int N = c.sum(d, r);
             if (4 * g < GR && 4 * g + r < rows) a.pN[(slot0 + 4 * g + r) * a.s.wide + 16 * d + n] = N;
         }
+}
+
+// The same where a block takes all the chunks of its row tile (J <= NEAR): their partial sums stay in LDS and are joined there
+#define NARROW_NEAR 4
+template <int BITS, int DK, int GR, int RU>
+__global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow_near(NarrowAtt a) {
+    using Chunk = NarrowChunk<BITS, DK, GR, RU>;
+    constexpr int WIDE = 64 * DK;
+    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
+    __shared__ __attribute__((aligned(16))) NarrowFew<DK, GR> few;
+    __shared__ int pN[NARROW_NEAR][GR][WIDE], pm[NARROW_NEAR][GR], pA[NARROW_NEAR][GR], pE[NARROW_NEAR][GR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int rt = blockIdx.x, h = blockIdx.y, stream = blockIdx.z, rows = a.R - rt * GR;
+    const i64 head = (i64)stream * a.s.heads + h;
+    int plo, phi;
+    if (!narrow_reach(a, stream, rt * GR, min(rt * GR + GR, a.R), plo, phi)) return;
+    narrow_few<DK, GR>(a, stream, h, rt, lane, wave, few);
+    static_assert(NARROW_NEAR == NTHREADS / 64, "a wave a chunk");
+    const int c0 = wave * NCHUNK;
+    if (c0 <= phi) {
+        Chunk c;
+        narrow_ready(c, few, rows, lane);
+        const char* base = a.buf + head * a.s.tiles * narrow_tile(a.s);
+        if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave]);
+        else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave]);
+        if (n == 0 && 4 * g < GR)
+#pragma unroll
+            for (int r = 0; r < RU; r++) { pm[wave][4 * g + r] = c.m[r]; pA[wave][4 * g + r] = c.A[r]; pE[wave][4 * g + r] = c.E[r]; }
+#pragma unroll
+        for (int d = 0; d < Chunk::DT; d++)
+#pragma unroll
+            for (int r = 0; r < RU; r++) {
+                const int N = c.sum(d, r);
+                if (4 * g < GR) pN[wave][4 * g + r][16 * d + n] = N;
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(GR, rows) * WIDE; i += NTHREADS) {
+        const int r = i / WIDE, d = i % WIDE, p = few.qp[r], J = p / NCHUNK + 1;
+        if (p < 0 || d >= a.s.dim) continue;
+        int M = pm[0][r], E = pE[0][r];
+        for (int j = 1; j < J; j++) { M = max(M, pm[j][r]); E = max(E, pE[j][r]); }
+        i64 A = 0, N = 0;
+        for (int j = 0; j < J; j++) {
+            const unsigned df = (unsigned)M - (unsigned)pm[j][r];
+            const i64 f = df < (unsigned)a.tb.alen ? a.tb.ARR[df] : 0;
+            A += rsh_round(pA[j][r] * f, 24);
+            N += rsh_round(pN[j][r][d] * f, min(24 + E - pE[j][r], 63));
+        }
+        const int rho = rt * GR + r, t = rho / a.group, hq = h * a.group + rho % a.group;
+        a.out[stream * a.o_stream + t * a.o_row + (i64)hq * a.s.dim + d] = power(N, ((i64)E + 8) * 65536 - log2fix(A, a.tb), a.tb);
+    }
 }
 
 // Many rows: a block 16 rows and all the positions that they see, its four waves every fourth chunk.  Scores: A = keys,
@@ -1248,8 +1314,16 @@ static void narrow_attend(const NarrowAtt& a, bool sweep, hipStream_t st) {
         launch(g_kt.stages, "narrow.sweep", k_narrow_sweep<BITS, DK>, dim3((unsigned)((a.R + 15) / 16), heads, streams), dim3(64 * SWEEP_WAVES), 0, st, a);
         return;
     }
-    const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, jb = (a.J + NTHREADS / 64 - 1) / (NTHREADS / 64);
-    const dim3 grid((unsigned)(jb * ((a.R + gr - 1) / gr)), heads, streams);
+    const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, rts = (a.R + gr - 1) / gr, jb = (a.J + NTHREADS / 64 - 1) / (NTHREADS / 64);
+    if (a.J <= NARROW_NEAR) {
+        auto near = [&](auto kern) { launch(g_kt.stages, "narrow.near", kern, dim3((unsigned)rts, heads, streams), dim3(NTHREADS), 0, st, a); };
+        if (a.R == 1) near(k_narrow_near<BITS, DK, 4, 1>);
+        else if (gr == 4) near(k_narrow_near<BITS, DK, 4, 4>);
+        else if (gr == 8) near(k_narrow_near<BITS, DK, 8, 4>);
+        else near(k_narrow_near<BITS, DK, 16, 4>);
+        return;
+    }
+    const dim3 grid((unsigned)(jb * rts), heads, streams);
     auto split = [&](auto kern) { launch(g_kt.stages, "narrow.split", kern, grid, dim3(NTHREADS), 0, st, a, jb); };
     if (a.R == 1) split(k_narrow_split<BITS, DK, 4, 1>);
     else if (gr == 4) split(k_narrow_split<BITS, DK, 4, 4>);

@@ -250,6 +250,52 @@ def test_many_rows(sm, dtabs, tabs, bits, dim, group, rows):
     attend(c, o, buf, dtabs, tabs, shape, rng, group, rows, [400, 200, 250, -200], None, 260)
 
 
+@pytest.mark.parametrize("bits,dim,group,rows,ctx", [(4, 64, 2, 17, 700), (8, 128, 1, 40, 600), (4, 256, 3, 20, 300), (8, 64, 1, 33, 1100),
+                                                     (4, 100, 1, 36, 530), (8, 200, 2, 18, 270), (4, 40, 5, 9, 1030)])
+def test_prompt_rows(sm, dtabs, tabs, bits, dim, group, rows, ctx):
+    """enough row tiles for the sweep: prompts of uneven lengths at uneven places, some not there at all"""
+    shape = (8, 12, dim, ctx, bits)
+    rng = np.random.default_rng(rows)
+    c, o, buf = filled_by_columns(sm, rng, shape)
+    start = [ctx - rows, 0, 250, -2, 5, ctx - 3, ctx + 5, 255]
+    attend(c, o, buf, dtabs, tabs, shape, rng, group, rows, start, [rows, 2, 0, 4, -1, rows, rows, 1], ctx)
+
+
+def filled_by_columns(sm, rng, shape):
+    """a cache written by one call, the heads of stream s > 0 sharing the values of two (the oracle's digits made once)"""
+    streams, heads, dim, ctx, bits = shape
+    c, o = sm.NarrowCache(*shape), orc.Cache(*shape)
+    some = [orc.Cache(1, 1, dim, ctx, bits) for _ in range(4)]
+    rows = [[rows_of(rng, (1, ctx, 1, dim), 12, 20) for _ in range(2)] for _ in some]
+    for x, (k, v) in zip(some, rows):
+        x.write(k, v, [0])
+    k, v = (np.zeros((streams, ctx, heads, dim), np.int64) for _ in range(2))
+    for s in range(streams):
+        for h in range(heads):
+            i = int(rng.integers(0, len(some)))
+            k[s, :, h], v[s, :, h] = rows[i][0][0, :, 0], rows[i][1][0, :, 0]
+            for name in ("k", "v", "kl", "vl"):
+                getattr(o, name)[s, h] = getattr(some[i], name)[0, 0]
+    buf, dk, dv, ds = torch.zeros(c.bytes, dtype=torch.uint8, device="cuda"), dev(k), dev(v), dev(np.zeros(streams, np.int32))
+    c.write(buf.data_ptr(), dk.data_ptr(), dv.data_ptr(), ctx, ds.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    return c, o, buf
+
+
+def test_sweep_levels_far_apart(sm, dtabs, tabs):
+    """test_levels_far_apart's keys, values and queries through the sweep"""
+    for shape in ((8, 12, 64, 300, 4), (8, 12, 128, 280, 8)):
+        rng = np.random.default_rng(shape[4])
+        c, o, buf = filled(sm, rng, (1, 1) + shape[2:], 0, 61)
+        one = buf.view(1, -1)
+        big, wide = sm.NarrowCache(*shape), orc.Cache(*shape)
+        for name in ("k", "v", "kl", "vl"):
+            getattr(wide, name)[:] = getattr(o, name)
+        for scale in (None, 0, -(64 << 16), 64 << 16, 77777):
+            attend(big, wide, one.expand(96, -1).contiguous(), dtabs, tabs, shape, rng, 1, 40, [240] * 8, [2, 0, 1, 0, 0, 0, 3, 0], shape[3],
+                   scale, 0, 61)
+
+
 def test_levels_far_apart(sm, dtabs, tabs):
     """keys, values and queries of any size: scores past every clamp, ties there, weights shifted out by the values' levels;
     scales from 2^-64 to 2^64"""
