@@ -109,6 +109,70 @@ SMD i64 narrow_out(int pile, int we, int sh, i64 wb) {
     return wadd(s > 31 ? 0 : (pile >> s) + ((pile >> (s - 1)) & 1), wb);
 }
 
+// Few values (rows ceil(K / 1024) <= 8): a block a column tile forms the rows' digits itself, in LDS, while its first weights
+// are on their way, and its four waves take a quarter of the inputs each.  One launch in place of two: a call is then
+// bound by its launch.
+constexpr int FEW_QUADS = 8;
+__global__ __launch_bounds__(NTHREADS) void k_narrow_one(Narrow8Args a) {
+    constexpr int AHEAD = 4;
+    __shared__ __attribute__((aligned(16))) signed char x8[FEW_QUADS * 1024];      // [K / 16][rows][16]
+    __shared__ u64 wor[FEW_QUADS][4];
+    __shared__ int lev[FEW_QUADS];
+    __shared__ v4i part[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int kbs = a.K / 64, per = (kbs + 3) / 4, k0 = wave * per, k1 = min(kbs, k0 + per), quads = a.K / 4;
+    const v4i* wp = reinterpret_cast<const v4i*>(a.W + (i64)blockIdx.x * a.K * 16) + lane;
+    v4i w[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+        if (k0 + i < k1) w[i] = wp[(k0 + i) * 64];
+    const int S = (quads + NTHREADS - 1) / NTHREADS, used = a.rows * S;
+    i64 v[FEW_QUADS][4];
+#pragma unroll
+    for (int i = 0; i < FEW_QUADS; i++) {
+        const int q = tid + i % S * NTHREADS;
+        if (i < used && q < quads) row_quad(a.X + (i64)(i / S) * a.ldx, q, a.nin, v[i]);
+        else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < FEW_QUADS; i++)
+        if (i < used) {
+            const u64 o = wave_or_u64(mag64(v[i][0]) | mag64(v[i][1]) | mag64(v[i][2]) | mag64(v[i][3]));
+            if (lane == 0) wor[i][wave] = o;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FEW_QUADS; i++) {
+        const int r = i / S, q = tid + i % S * NTHREADS;
+        if (i >= used) continue;
+        u64 o = 0;
+        for (int j = r * S; j < (r + 1) * S; j++) o |= wor[j][0] | wor[j][1] | wor[j][2] | wor[j][3];
+        const int sh = digit_level(o, 8);
+        if (tid == 0) lev[r] = sh;
+        if (q >= quads) continue;
+        unsigned d = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) d |= (unsigned)(digit_of(v[i][j], sh, 8) & 255) << (8 * j);
+        *reinterpret_cast<unsigned*>(x8 + ((q >> 2) * a.rows + r) * 16 + 4 * (q & 3)) = d;
+    }
+    __syncthreads();
+    v4i acc = {};
+    const signed char* xr = x8 + min(n, a.rows - 1) * 16;
+    for (int k = k0; k < k1; k += AHEAD)
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (k + i < k1) {
+                acc = mfma8(*reinterpret_cast<const v4i*>(xr + (4 * (k + i) + g) * a.rows * 16), w[i], acc);
+                if (k + i + AHEAD < k1) w[i] = wp[(k + i + AHEAD) * 64];
+            }
+    part[wave][lane] = acc;
+    __syncthreads();
+    const int col = blockIdx.x * 16 + n, row = 4 * g + wave;               // wave w finishes every fourth row
+    if (col >= a.N || row >= a.rows) return;
+    const int pile = part[0][lane][wave] + part[1][lane][wave] + part[2][lane][wave] + part[3][lane][wave];
+    a.out[(i64)row * a.ldo + col] = narrow_out(pile, a.we[col], lev[row], a.wb[col]);
+}
+
 // RT row tiles by CT column tiles a wave, the inputs split over KW of a block's four waves and their piles added
 template <int RT, int CT, int KW>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
@@ -123,18 +187,26 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
 #pragma unroll
     for (int r = 0; r < RT; r++) lp[r] = reinterpret_cast<const v4i*>(a.lights + (i64)min(rt0 + r, rts - 1) * a.K * 16) + lane;
     v4i acc[RT][CT] = {};
-#pragma unroll 4
-    for (int k = k0; k < k1; k++) {
-        v4i w[CT], x[RT];
+    auto steps = [&](int k, auto many) {
+        constexpr int U = decltype(many)::value;
+        v4i w[U][CT], x[U][RT];
 #pragma unroll
-        for (int c = 0; c < CT; c++) w[c] = wp[c][k * 64];
+        for (int i = 0; i < U; i++) {
 #pragma unroll
-        for (int r = 0; r < RT; r++) x[r] = lp[r][k * 64];
+            for (int c = 0; c < CT; c++) w[i][c] = wp[c][(k + i) * 64];
 #pragma unroll
-        for (int r = 0; r < RT; r++)
+            for (int r = 0; r < RT; r++) x[i][r] = lp[r][(k + i) * 64];
+        }
 #pragma unroll
-            for (int c = 0; c < CT; c++) acc[r][c] = mfma8(x[r], w[c], acc[r][c]);
-    }
+        for (int i = 0; i < U; i++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int c = 0; c < CT; c++) acc[r][c] = mfma8(x[i][r], w[i][c], acc[r][c]);
+    };
+    int k = k0;
+    for (; k + 4 <= k1; k += 4) steps(k, std::integral_constant<int, 4>());
+    for (; k < k1; k++) steps(k, std::integral_constant<int, 1>());
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -446,16 +518,17 @@ SMD int narrow_pos(const NarrowAtt& a, int stream, int t) {
     const i64 p = (i64)a.start[stream] + t;
     return t < (a.count ? a.count[stream] : a.rows) && p >= 0 && p < a.span ? (int)p : -1;
 }
-// one wave: the 8-bit digits of one row's q (zeros past its dimension, and for a row that is not there) and their level
+// one wave: one row's q (zeros past its dimension, and for a row that is not there), its 8-bit digits and their level
 template <int PER>
-SMD int narrow_q_row(const NarrowAtt& a, const i64* q, bool here, int lane, signed char* dst) {
-    i64 x[PER];
+SMD void narrow_q_load(const NarrowAtt& a, const i64* q, bool here, int lane, i64 x[PER]) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) x[j] = here && lane + 64 * j < a.s.dim ? q[lane + 64 * j] : 0;
+}
+template <int PER>
+SMD int narrow_q_row(const NarrowAtt& a, i64 x[PER], int lane, signed char* dst) {
     u64 o = 0;
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        x[j] = here && lane + 64 * j < a.s.dim ? q[lane + 64 * j] : 0;
-        o |= mag64(x[j]);
-    }
+    for (int j = 0; j < PER; j++) o |= mag64(x[j]);
     const int s16 = digit_level(wave_or_u64(o), 16);
     const i64 e = a.tb.EXP2[a.F & 0xFFFF];
     o = 0;
@@ -479,7 +552,9 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_q(NarrowAtt a) {
     const int t = i / q_heads, hq = i % q_heads, h = hq / a.group, rho = t * a.group + hq % a.group;
     const i64 slot = ((i64)stream * a.s.heads + h) * a.R + rho;
     const int p = narrow_pos(a, stream, t);
-    const int eq = narrow_q_row<PER>(a, a.q + stream * a.q_stream + t * a.q_row + (i64)hq * a.s.dim, p >= 0, lane, a.q8 + slot * a.s.wide);
+    i64 x[PER];
+    narrow_q_load<PER>(a, a.q + stream * a.q_stream + t * a.q_row + (i64)hq * a.s.dim, p >= 0, lane, x);
+    const int eq = narrow_q_row<PER>(a, x, lane, a.q8 + slot * a.s.wide);
     if (lane == 0) { a.pos[slot] = p; a.eq[slot] = eq; }
 }
 
@@ -556,11 +631,14 @@ SMD void value_operands(v4i x, v4i out[8 / BITS]) {
 // A score: dot 2^e rounded half up, held to 32 bits (v_cvt_rpi_i32_f32: floor(x + 1/2), saturating; dot has at most 23
 // bits, so dot 2^e is exact in float).  Compared with that function in whole numbers for every dot and every e from -60 to
 // 100: equal.
-SMD int narrow_score(int dot, int e) {
-    int s;
-    asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(s) : "v"(ldexpf((float)dot, e)));
+// (The compiler's wait states around the matrix units do not know what an asm block writes, so these write the register
+// they read: whatever the matrix units still read or write there was waited for by the instruction before.)
+SMD int narrow_round(float x) {
+    int s = __builtin_bit_cast(int, x);
+    asm("v_cvt_rpi_i32_f32 %0, %0" : "+v"(s));
     return s;
 }
+SMD int narrow_score(int dot, int e) { return narrow_round(ldexpf((float)dot, e)); }
 // the exponent that a key's level is added to (past 40 every dot but 0 is clamped all the same)
 template <int BITS> SMD int narrow_exp(int eq) { return min(eq - 6 - (BITS == 4 ? 4 : 0), 40); }      // (4-bit operands are 16 times the digit)
 // Scores are clamped to +-2^30 where they are compared: m is clamped, and a score's distance to it is held to 0 .. far with
@@ -569,8 +647,8 @@ template <int BITS> SMD int narrow_exp(int eq) { return min(eq - 6 - (BITS == 4 
 SMD int narrow_clamp(int m) { return min(max(m, -(1 << 30)), 1 << 30); }
 SMD int narrow_far(int m, int alen) { return (int)min((unsigned)alen, (unsigned)max(m, -(1 << 30)) + (1u << 30)); }      // (2^31 at m 2^30)
 SMD int narrow_distance(int m, int s, int far) {
-    int d;
-    asm("v_med3_i32 %0, %1, 0, %2" : "=v"(d) : "v"(__builtin_elementwise_sub_sat(m, s)), "v"(far));
+    int d = __builtin_elementwise_sub_sat(m, s);
+    asm("v_med3_i32 %0, %0, 0, %1" : "+v"(d) : "v"(far));
     return d;
 }
 // A weight w in 0 .. 2^22 (u shifted by the levels' distance) as three signed bytes b0 + 256 b1 + 65536 b2: w + 0x808080
@@ -729,10 +807,22 @@ SMD bool narrow_reach(const NarrowAtt& a, int stream, int first, int end, int& p
 }
 template <int DK, int GR>
 SMD void narrow_few(const NarrowAtt& a, int stream, int h, int rt, int lane, int wave, NarrowFew<DK, GR>& f) {
-    for (int r = wave; r < min(GR, a.R - rt * GR); r += NTHREADS / 64) {
-        const int rho = rt * GR + r, t = rho / a.group, p = narrow_pos(a, stream, t);
-        const int e = narrow_q_row<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p >= 0, lane, f.qd[r]);
-        if (lane == 0) { f.qe[r] = e; f.qp[r] = p; }
+    constexpr int PER = GR * 64 / NTHREADS;                          // a wave's rows: loaded together
+    const int rows = min(GR, a.R - rt * GR);
+    i64 x[PER][DK];
+    int p[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = wave + i * (NTHREADS / 64), rho = rt * GR + r, t = rho / a.group;
+        p[i] = r < rows ? narrow_pos(a, stream, t) : -1;
+        narrow_q_load<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p[i] >= 0, lane, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = wave + i * (NTHREADS / 64);
+        if (r >= rows) break;
+        const int e = narrow_q_row<DK>(a, x[i], lane, f.qd[r]);
+        if (lane == 0) { f.qe[r] = e; f.qp[r] = p[i]; }
     }
     __syncthreads();
 }
@@ -920,8 +1010,7 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
             else look(std::false_type());
             if ((T & 3) == 3 || T == last) {
                 const int j = T >> 2;
-                int mi;
-                asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(mi) : "v"(m));
+                int mi = narrow_round(m);
                 mi = max_g(j * NCHUNK + 4 * g <= pos ? narrow_clamp(mi) : NARROW_NONE);
                 e = max_g(e);
                 if (g == 0) { pm[(i64)j * a.R] = mi; pE[(i64)j * a.R] = e; }
@@ -1191,6 +1280,11 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     a.lights = static_cast<signed char*>(work);
     a.level = reinterpret_cast<int*>(static_cast<char*>(work) + plate8_lights(p, rows));
     hipStream_t s = (hipStream_t)stream;
+    if ((i64)rows * ((p->K + 1023) / 1024) <= FEW_QUADS) {
+        launch(g_kt.stages, "plate8.one", k_narrow_one, dim3((unsigned)((a.N + 15) / 16)), dim3(NTHREADS), 0, s, a);
+        HIP_TRY(hipGetLastError());
+        return SM_OK;
+    }
     launch(g_kt.stages, "plate8.lights", k_narrow_lights, dim3((unsigned)(rows < 128 ? rows : (rows + 127) / 128 * 128)), dim3(NTHREADS), 0, s, a);
     const int nt = (a.N + 15) / 16, rts = (rows + 15) / 16;
     if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
