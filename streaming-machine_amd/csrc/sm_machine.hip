@@ -22,6 +22,7 @@
 #include <cstring>
 #include <fstream>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cxxabi.h>
 #include <map>
@@ -282,7 +283,10 @@ static void free_mfma_plate(MfmaPlate& P) {
 struct sm_tables {
     int* LOG2 = nullptr; int* EXP2 = nullptr; int* PHI = nullptr; int* ARR = nullptr;
     int* GPOW = nullptr; int* HPOW = nullptr; int* PGPOW = nullptr;
-    int* ARR2 = nullptr;      // [alen + 1] 2 rsh(ARR[d], 2), a 0 at the end: the narrow attention's weights
+    // the narrow attention's: [alen + 1] 2 rsh(ARR[d], 2), a 0 at the end; e^(-d / 8) 2^24 for d <= alen / 128, then
+    // e^(-d / 1024) for d < 128, where their product rounds to ARR[d] for every d up to alen (else null)
+    int* ARR2 = nullptr;
+    double* ARRF = nullptr;
     int alen = 0;
     i64 log768 = 0, eps40 = 0;
     int verified = 0;         // every entry equals its defining formula (checked on the device at create)
@@ -321,6 +325,16 @@ static int tables_init(sm_tables& T, const i64* phi, const i64* arr, int alen, c
         std::vector<i64> w(alen + 1, 0);
         for (int d = 0; d < alen; d++) w[d] = (arr[d] + 2) >> 2 << 1;
         if ((rc = upload_table(&T.ARR2, w.data(), w.size(), 0, 1 << 23, "arrival weights"))) return rc;
+        std::vector<double> f(alen / 128 + 1 + 128);
+        for (int d = 0; d <= alen / 128; d++) f[d] = std::exp(-d / 8.0) * 16777216.0;
+        for (int d = 0; d < 128; d++) f[alen / 128 + 1 + d] = std::exp(-d / 1024.0);
+        bool same = true;
+        for (int d = 0; d <= alen && same; d++)
+            same = std::fma(f[d / 128], f[alen / 128 + 1 + d % 128], 6755399441055744.0) - 6755399441055744.0 == (d < alen ? (double)arr[d] : 0.0);
+        if (same) {
+            if ((rc = dalloc(&T.ARRF, f.size()))) return rc;
+            HIP_TRY(hipMemcpy(T.ARRF, f.data(), f.size() * 8, hipMemcpyHostToDevice));
+        }
     }
     if ((rc = upload_table(&T.LOG2, log2t, 65536, 0, 65536, "log2"))) return rc;
     if ((rc = upload_table(&T.EXP2, exp2t, 65536, 65536, 131072, "exp2"))) return rc;
@@ -366,7 +380,7 @@ static int stage_init(sm_tables& T) {
 }
 
 static void tables_free(sm_tables& T) {
-    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.ARR2); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
+    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.ARR2); hfree(T.ARRF); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
     hfree(T.asc); hfree(T.acm); hfree(T.aacc); hfree(T.posn);
     if (T.herr) (void)hipHostFree(T.herr);
 }

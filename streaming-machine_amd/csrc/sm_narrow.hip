@@ -510,6 +510,7 @@ struct NarrowAtt {
     int* eq; int* pos;           // [streams][heads][R] the digits' level; the row's position, -1 a row that is not there
     int* pm; int* pA; int* pE; int* pN;     // [streams][heads][J][R] each chunk's m_j, A_j, E_j and (x wide) N_j
     const int* W2;               // the arrivals' weights 2 rsh(ARR[d], 2), 0 at alen
+    const double* WF;            // ARR's factors (sm_tables): [alen / 128 + 1], [128]
     Tables tb;
 };
 
@@ -660,6 +661,24 @@ template <int BITS> SMD int narrow_sum(int n0, int n1, int n2) {
     return BITS == 8 ? q + ((n0 + 128) >> 8) : (q + ((n0 + 2048) >> 8)) >> 4;
 }
 
+// The arrivals as products of two short tables in LDS: ARR[d] = rint(e^(-(d / 128) / 8) 2^24 e^(-(d % 128) / 1024)), which the
+// tables' creation has compared with every entry.  2^52 + 2^51 + 2 added in the same step leaves ARR[d] + 2 in the low word,
+// and 2 rsh(ARR[d], 2) is that without its last two bits, halved.  (Gathered from the 71 KB table in memory, the weights
+// took 33 us of the 106 that 64 streams of up to 8,192 positions spent in this kernel.)
+#define NARROW_H 140
+#define SWEEP_ARR 17790            // entries of the arrival that the kernels hold (base2_convert.py:50-53 gives 17,745)
+struct NarrowFactors {
+    double h[NARROW_H], l[128];
+    SMD void load(const NarrowAtt& a, int tid) {
+        const int nh = a.tb.alen / 128 + 1;
+        for (int i = tid; i < nh + 128; i += NTHREADS) (i < nh ? h[i] : l[i - nh]) = a.WF[i];
+    }
+    SMD int weight(int d) const {
+        const double x = __builtin_fma(h[d >> 7], l[d & 127], 6755399441055746.0);
+        return (int)((unsigned)__builtin_bit_cast(u64, x) >> 1 & ~1u);
+    }
+};
+
 // Few rows: a wave a chunk, a tile of GR rows (RU of every four wanted).  Scores: A = q, B = keys, so a lane is a position.
 // With fewer than 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position
 // tiles add into one accumulator: every lane then holds a score that is wanted.  Weights: byte planes through the wave's
@@ -676,13 +695,13 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
     // base: the head's tiles; c0: the chunk's first position; last: the last tile that holds a position seen; whole: every
     // row sees all 256
     template <bool WHOLE>
-    SMD void run(const NarrowAtt& a, const char* base, int c0, int last, int lane, unsigned char* wb) {
+    SMD void run(const NarrowAtt& a, const char* base, int c0, int last, int lane, unsigned char* wb, const NarrowFactors& wf) {
         const int n = lane & 15, g = lane >> 4, t0 = c0 / 64;
         const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
         auto tile = [&](int t) { return base + (i64)min(t0 + t, last) * tile_bytes; };
         KeyRaw<BITS, DK> k[4][4];
         v4i v[4][DT / VU];
-        int kl[4][NA], vl[4][NA];
+        int lev[4];
         auto load_k = [&](int t) {
 #pragma unroll
             for (int sub = 0; sub < 4; sub++) k[t][sub].load(tile(t), sub, n, g);
@@ -691,15 +710,11 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
 #pragma unroll
             for (int c = 0; c < DT / VU; c++) v[t][c] = *reinterpret_cast<const v4i*>(tile(t) + half + c * 1024 + lane * 16);
         };
+        // a tile's 128 levels are one line: one load of it
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const unsigned char* lev = reinterpret_cast<const unsigned char*>(tile(t) + 2 * half);
-#pragma unroll
-            for (int x = 0; x < NA; x++) {
-                kl[t][x] = lev[16 * (x * PT + 4 * g / GR) + n];
-                vl[t][x] = lev[64 + 16 * (x * PT + 4 * g / GR) + n];
-            }
-        }
+        for (int t = 0; t < 4; t++) lev[t] = reinterpret_cast<const int*>(tile(t) + 2 * half)[lane & 31];
+        int vl[4][NA];
+        auto level = [&](int t, int at) { return (int)((unsigned)__shfl(lev[t], at >> 2, 64) >> 8 * (at & 3) & 255u); };
 #pragma unroll
         for (int t = 0; t < AHEAD; t++) load_k(t);
         int sc[4][NA][RU];
@@ -719,10 +734,11 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
             }
 #pragma unroll
             for (int x = 0; x < NA; x++) {
-                const int i = c0 + 64 * t + 16 * (x * PT + 4 * g / GR) + n;
+                const int at = 16 * (x * PT + 4 * g / GR) + n, i = c0 + 64 * t + at, kl = level(t, at);
+                vl[t][x] = level(t, 64 + at);
 #pragma unroll
                 for (int r = 0; r < RU; r++) {
-                    sc[t][x][r] = narrow_score(acc[x][r], er[r] + kl[t][x]);
+                    sc[t][x][r] = narrow_score(acc[x][r], er[r] + kl);
                     m[r] = WHOLE || i <= pos[r] ? max(m[r], sc[t][x][r]) : m[r];
                     if (!WHOLE || r == 0) E[r] = max(E[r], WHOLE || i <= pos[r] ? vl[t][x] : 0);
                 }
@@ -758,7 +774,7 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
                         if (c0 + 64 * t + 16 * T + n > pos[r]) d = a.tb.alen;
                         sh = max(sh, 0);
                     }
-                    const int u2 = a.W2[d];
+                    const int u2 = wf.weight(d);
                     A[r] += u2;
                     const unsigned b = narrow_weight(u2, sh) ^ 0x808080u;
                     const int row0 = (4 * g + r) % GR;
@@ -795,6 +811,7 @@ template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
 // What the blocks of few rows begin with: the positions of the tile's first and last row (a row that is not there takes no
 // part), and the rows' digits, levels and positions in LDS
 template <int DK, int GR> struct NarrowFew {
+    NarrowFactors wf;
     signed char qd[GR][64 * DK];
     int qe[GR], qp[GR];
 };
@@ -809,6 +826,7 @@ template <int DK, int GR>
 SMD void narrow_few(const NarrowAtt& a, int stream, int h, int rt, int lane, int wave, NarrowFew<DK, GR>& f) {
     constexpr int PER = GR * 64 / NTHREADS;                          // a wave's rows: loaded together
     const int rows = min(GR, a.R - rt * GR);
+    f.wf.load(a, wave * 64 + lane);
     i64 x[PER][DK];
     int p[PER];
 #pragma unroll
@@ -856,8 +874,8 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
     Chunk c;
     narrow_ready(c, few, rows, lane);
     const char* base = a.buf + head * a.s.tiles * narrow_tile(a.s);
-    if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave]);
-    else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave]);
+    if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave], few.wf);
+    else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave], few.wf);
     const i64 slot0 = (head * a.J + j) * a.R + rt * GR;
     if (n == 0 && 4 * g < GR)
 #pragma unroll
@@ -887,14 +905,15 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
     int plo, phi;
     if (!narrow_reach(a, stream, rt * GR, min(rt * GR + GR, a.R), plo, phi)) return;
     narrow_few<DK, GR>(a, stream, h, rt, lane, wave, few);
+    static_assert((SWEEP_ARR + 1) / 128 + 1 <= NARROW_H, "the arrival's factors fit");
     static_assert(NARROW_NEAR == NTHREADS / 64, "a wave a chunk");
     const int c0 = wave * NCHUNK;
     if (c0 <= phi) {
         Chunk c;
         narrow_ready(c, few, rows, lane);
         const char* base = a.buf + head * a.s.tiles * narrow_tile(a.s);
-        if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave]);
-        else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave]);
+        if (c0 + NCHUNK - 1 <= plo) c.template run<true>(a, base, c0, phi / 64, lane, wbuf[wave], few.wf);
+        else c.template run<false>(a, base, c0, phi / 64, lane, wbuf[wave], few.wf);
         if (n == 0 && 4 * g < GR)
 #pragma unroll
             for (int r = 0; r < RU; r++) { pm[wave][4 * g + r] = c.m[r]; pA[wave][4 * g + r] = c.A[r]; pE[wave][4 * g + r] = c.E[r]; }
@@ -929,7 +948,6 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
 // weight operand are (the values' layout): nothing moves between lanes.  A first pass over the keys finds each chunk's m_j
 // and E_j (kept in memory) and the row's M and E; the second adds each chunk's N_j f_j in registers, and the waves' sums are
 // added at the end.  Bound by the vector arithmetic of a score, so the arrivals' weights stand in LDS.
-#define SWEEP_ARR 17919            // entries of the arrival that fit (base2_convert.py:50-53 gives 17,745)
 #define SWEEP_WAVES 4
 template <int BITS, int DK>
 __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sweep(NarrowAtt a) {
@@ -963,14 +981,15 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
     };
     // a tile's keys and levels, and its values; each register takes the next tile's as soon as it has been used
     KeyRaw<BITS, DK> k[4];
-    int kl[4], vl[4];
+    int lev;                                                         // (one load of the line: see NarrowChunk)
     v4i v[DT / VU];
     auto load_sub = [&](int T, int sub) {
         const char* tp = base + (i64)T * tile_bytes;
         k[sub].load(tp, sub, n, g);
-        kl[sub] = reinterpret_cast<const int*>(tp + 2 * half)[4 * sub + g];
-        vl[sub] = reinterpret_cast<const int*>(tp + 2 * half)[16 + 4 * sub + g];
+        if (sub == 3) lev = reinterpret_cast<const int*>(tp + 2 * half)[lane & 31];
     };
+    auto key_levels = [&](int sub) { return __shfl(lev, 4 * sub + g, 64); };
+    auto value_levels = [&](int sub) { return __shfl(lev, 16 + 4 * sub + g, 64); };
     auto load_v = [&](int T, int c) { v[c] = *reinterpret_cast<const v4i*>(base + (i64)T * tile_bytes + half + c * 1024 + lane * 16); };
     auto after = [](int T) { return (T & 3) == 3 ? T + 4 * NW - 3 : T + 1; };
     // dots of the 16 positions of a sub-tile with the lane's row, positions 4 g .. 4 g + 3 of it
@@ -996,7 +1015,7 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
 #pragma unroll
                 for (int sub = 0; sub < 4; sub++) {
                     const v4i acc = dots(sub);
-                    const int l = kl[sub], lv = vl[sub];
+                    const int l = key_levels(sub), lv = value_levels(sub);
                     load_sub(Tn, sub);
 #pragma unroll
                     for (int r = 0; r < 4; r++)
@@ -1050,7 +1069,7 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
 #pragma unroll
                 for (int sub = 0; sub < 4; sub++) {
                     const v4i acc = dots(sub);
-                    const int l = kl[sub], lv = vl[sub];
+                    const int l = key_levels(sub), lv = value_levels(sub);
                     load_sub(have, sub);
                     unsigned x[4];
 #pragma unroll
@@ -1445,7 +1464,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     if ((i64)((a.J + 3) / 4) * ((a.R + 3) / 4) > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_attend: too many rows at this span for one call");
     const NarrowWork w = narrow_work(a.s, a.R, a.J);
     if (work_bytes < w.bytes) return fail(SM_E_ARG, "sm_narrow_attend: the workspace is smaller than sm_narrow_work");
-    if (t->alen > SWEEP_ARR) return fail(SM_E_ARG, "sm_narrow_attend: the tables' arrival has more entries than the kernels hold");
+    if (!t->ARRF || t->alen > SWEEP_ARR) return fail(SM_E_ARG, "sm_narrow_attend: the tables' arrival is not base2_convert.py's");
     OnDevice on(buf);
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_attend: the cache is not in a device's memory");
     char* wk = static_cast<char*>(work);
@@ -1453,7 +1472,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     a.q = (const i64*)q; a.q_row = q_row; a.q_stream = q_stream; a.out = (i64*)out; a.o_row = out_row; a.o_stream = out_stream;
     a.start = start; a.count = count; a.span = span; a.F = scale; a.tb = t->tb();
     a.q8 = reinterpret_cast<signed char*>(wk + w.q8); a.eq = reinterpret_cast<int*>(wk + w.eq); a.pos = reinterpret_cast<int*>(wk + w.pos);
-    a.pm = reinterpret_cast<int*>(wk + w.pm); a.W2 = t->ARR2; a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
+    a.pm = reinterpret_cast<int*>(wk + w.pm); a.W2 = t->ARR2; a.WF = t->ARRF; a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
     a.pN = reinterpret_cast<int*>(wk + w.pN);
     hipStream_t st = (hipStream_t)stream;
     if (a.s.bits == 4) a.s.wide == 64 ? narrow_attend<4, 1>(a, w.sweep, st) : a.s.wide == 128 ? narrow_attend<4, 2>(a, w.sweep, st) : narrow_attend<4, 4>(a, w.sweep, st);
