@@ -20,6 +20,13 @@ SMD int digit_of(i64 x, int sh, int bits) {
     const i64 v = rsh_round(x, sh), hi = (1 << (bits - 1)) - 1;
     return (int)(v > hi ? hi : v < -hi - 1 ? -hi - 1 : v);
 }
+// the same digits of a row whose level shows that its values fit 32 bits (sh < 32 - bits; the low words then hold them): four
+// steps a value in place of some twenty of 64 bits.  Only the upper end is ever clamped.
+SMD int digit_short(int x, int sh, int bits) {
+    const int v = (x >> sh) + (int)(sh ? __builtin_amdgcn_ubfe((unsigned)x, (unsigned)sh - 1, 1) : 0);
+    return min(v, (1 << (bits - 1)) - 1);
+}
+SMD bool digits_short(int sh, int bits) { return sh < 32 - bits; }
 SMD u64 mag64(i64 x) { return x < 0 ? (u64)0 - (u64)x : (u64)x; }
 // the OR over a wave of 64-bit values, in every lane
 SMD u64 wave_or_u64(u64 v) { return (u64)wave_or64((i64)v); }
@@ -36,6 +43,18 @@ struct Narrow8Args {
     i64* out; i64 ldo;
 };
 
+// four digits of a row as bytes
+SMD unsigned digit_quad(const i64 v[4], int sh) {
+    unsigned w = 0;
+    if (digits_short(sh, 8)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (unsigned)(digit_short((int)v[i], sh, 8) & 255) << (8 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (unsigned)(digit_of(v[i], sh, 8) & 255) << (8 * i);
+    }
+    return w;
+}
 // four values of a row from place 4 q, zeros past its end (rows stand at 8 bytes' alignment only)
 typedef i64 i64x2 __attribute__((ext_vector_type(2), aligned(8)));
 SMD void row_quad(const i64* x, int q, int nin, i64 v[4]) {
@@ -85,11 +104,8 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
     if (tid == 0) a.level[r] = sh;
     signed char* o = a.lights + (i64)(r >> 4) * a.K * 16 + (r & 15) * 16;
     auto store = [&](int q, const i64 v[4]) {
-        unsigned w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w |= (unsigned)(digit_of(v[i], sh, 8) & 255) << (8 * i);
         const int k = 4 * q;
-        *reinterpret_cast<unsigned*>(o + (i64)(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 15)) = w;
+        *reinterpret_cast<unsigned*>(o + (i64)(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 15)) = digit_quad(v, sh);
     };
 #pragma unroll
     for (int s = 0; s < HOLD; s++)
@@ -150,10 +166,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_one(Narrow8Args a) {
         const int sh = digit_level(o, 8);
         if (tid == 0) lev[r] = sh;
         if (q >= quads) continue;
-        unsigned d = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) d |= (unsigned)(digit_of(v[i][j], sh, 8) & 255) << (8 * j);
-        *reinterpret_cast<unsigned*>(x8 + ((q >> 2) * a.rows + r) * 16 + 4 * (q & 3)) = d;
+        *reinterpret_cast<unsigned*>(x8 + ((q >> 2) * a.rows + r) * 16 + 4 * (q & 3)) = digit_quad(v[i], sh);
     }
     __syncthreads();
     v4i acc = {};
@@ -370,12 +383,13 @@ SMD void narrow_range(const int* start, const int* count, int stream, int rows, 
     hi = min(hi, (i64)ctx - p0);
 }
 
-// a block a (tile, head, stream): its rows' levels and digits (a wave a row) through LDS, then whole 16-byte units; a
-// unit of values is read first where it also holds positions that the call does not write
+// A block a (tile, head, stream): its rows' levels and digits (a wave a row, four rows' loads in flight), through LDS in the
+// units' order (a dimension's positions 16 t + 4 g + r at byte 16 g + 4 t + r), then whole 16-byte units; a unit of values is
+// read first where it also holds positions that the call does not write.  Bound by the rows' read.
 template <int BITS, int WIDE>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
-    constexpr int PER = WIDE / 64;
-    __shared__ __attribute__((aligned(16))) signed char kd[64][WIDE + 4], vd[64][WIDE + 4];
+    constexpr int PER = WIDE / 64, AT_ONCE = PER == 4 ? 2 : 4, NW = NTHREADS / 64;
+    __shared__ __attribute__((aligned(16))) signed char kd[64][WIDE + 4], vd[WIDE][68];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, stream = blockIdx.z;
     i64 p0, lo, hi;
     narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
@@ -386,105 +400,126 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
     const int b0 = (int)max(first - tile * 64, (i64)0), b1 = (int)min(last - tile * 64, (i64)63);    // within the tile
     char* base = narrow_at(a.buf, a.s, stream, head, (int)tile);
     char* lev = base + 2 * narrow_half(a.s);
-    for (int b = b0 + wave; b <= b1; b += NTHREADS / 64) {
-        const i64 row = tile * 64 + b - p0, at = stream * a.stream_stride + row * a.row_stride + (i64)head * a.s.dim;
-        i64 xk[PER], xv[PER];
-        u64 ok = 0, ov = 0;
+    const i64 row0 = tile * 64 - p0, at0 = stream * a.stream_stride + (i64)head * a.s.dim;
+    for (int b = b0 + wave; b <= b1; b += NW * AT_ONCE) {
+        i64 x[AT_ONCE][2][PER];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int d = lane + 64 * i;
-            xk[i] = d < a.s.dim ? a.k[at + d] : 0;
-            xv[i] = d < a.s.dim ? a.v[at + d] : 0;
-            ok |= mag64(xk[i]);
-            ov |= mag64(xv[i]);
-        }
-        const int sk = digit_level(wave_or_u64(ok), BITS), sv = digit_level(wave_or_u64(ov), BITS);
+        for (int i = 0; i < AT_ONCE; i++) {
+            const i64 at = at0 + (row0 + min(b + i * NW, b1)) * a.row_stride;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            kd[b][lane + 64 * i] = (signed char)digit_of(xk[i], sk, BITS);
-            vd[b][lane + 64 * i] = (signed char)digit_of(xv[i], sv, BITS);
+            for (int j = 0; j < PER; j++) {
+                const int d = lane + 64 * j;
+                x[i][0][j] = d < a.s.dim ? a.k[at + d] : 0;
+                x[i][1][j] = d < a.s.dim ? a.v[at + d] : 0;
+            }
         }
-        if (lane == 0) { lev[b] = (char)sk; lev[64 + b] = (char)sv; }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int p = b + i * NW;
+            if (p > b1) break;
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                u64 o = 0;
+#pragma unroll
+                for (int j = 0; j < PER; j++) o |= mag64(x[i][kv][j]);
+                const int sh = digit_level(wave_or_u64(o), BITS);
+                if (lane == 0) lev[64 * kv + p] = (char)sh;
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const int v = digits_short(sh, BITS) ? digit_short((int)x[i][kv][j], sh, BITS) : digit_of(x[i][kv][j], sh, BITS);
+                    if (kv == 0) kd[p][lane + 64 * j] = (signed char)v;
+                    else vd[lane + 64 * j][16 * (p >> 2 & 3) + 4 * (p >> 4) + (p & 3)] = (signed char)v;
+                }
+            }
+        }
     }
     __syncthreads();
+    // the 4-bit digits of two dwords of bytes, the second ones in the high halves
+    auto halves = [](int x, int y) { return (int)(((unsigned)x & 0x0F0F0F0Fu) | ((unsigned)y & 0x0F0F0F0Fu) << 4); };
     constexpr int UNITS = WIDE * BITS / 128;                     // 16-byte units a position, or a dimension's 64 / 4
+    const bool whole = b0 == 0 && b1 == 63;
     for (int i = tid; i < UNITS * 64; i += NTHREADS) {
         const int c = i >> 6, b = i & 63;
         if (b < b0 || b > b1) continue;
-        unsigned w[4];
+        const int* row = reinterpret_cast<const int*>(kd[b]);
+        v4i w;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            w[q] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const unsigned v = BITS == 8 ? (unsigned)kd[b][16 * c + 4 * q + j] & 255u
-                    : ((unsigned)kd[b][32 * c + 4 * q + j] & 15u) | ((unsigned)kd[b][32 * c + 16 + 4 * q + j] & 15u) << 4;
-                w[q] |= v << (8 * j);
-            }
-        }
-        *reinterpret_cast<v4i*>(base + (i64)i * 16) = v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+        for (int q = 0; q < 4; q++) w[q] = BITS == 8 ? row[4 * c + q] : halves(row[8 * c + q], row[8 * c + 4 + q]);
+        *reinterpret_cast<v4i*>(base + (i64)i * 16) = w;
     }
     char* vbase = base + narrow_half(a.s);
     for (int i = tid; i < UNITS * 64; i += NTHREADS) {
         const int c = i >> 6, g = (i >> 4) & 3, m = i & 15;
-        // the unit's positions 16 t + 4 g + r: which of them the call writes
-        unsigned in = 0;
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int p = 16 * (j >> 2) + 4 * g + (j & 3);
-            in |= (p >= b0 && p <= b1 ? 1u : 0u) << j;
-        }
-        if (!in) continue;
-        v4i* u = reinterpret_cast<v4i*>(vbase + (i64)i * 16);
-        v4i old = {};
-        if (in != 0xFFFFu) old = *u;
+        v4i w;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            unsigned w = 0, keep = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (BITS == 8) {
-                    const int p = 16 * q + 4 * g + j;
-                    w |= ((unsigned)vd[p][16 * c + m] & 255u) << (8 * j);
-                    keep |= (in >> (4 * q + j) & 1 ? 0u : 255u) << (8 * j);
-                } else {
-                    const int t = q & 1, p = 16 * t + 4 * g + j, d = 32 * c + 16 * (q >> 1) + m;
-                    w |= (((unsigned)vd[p][d] & 15u) | ((unsigned)vd[p + 32][d] & 15u) << 4) << (8 * j);
-                    keep |= ((in >> (4 * t + j) & 1 ? 0u : 15u) | (in >> (4 * t + 8 + j) & 1 ? 0u : 240u)) << (8 * j);
-                }
-            }
-            old[q] = (int)((w & ~keep) | ((unsigned)old[q] & keep));
+            const int* row = reinterpret_cast<const int*>(vd[BITS == 8 ? 16 * c + m : 32 * c + 16 * (q >> 1) + m]) + 4 * g;
+            w[q] = BITS == 8 ? row[q] : halves(row[q & 1], row[(q & 1) + 2]);
         }
-        *u = old;
+        v4i* u = reinterpret_cast<v4i*>(vbase + (i64)i * 16);
+        if (!whole) {
+            // the unit's positions 16 t + 4 g + r: which of them the call writes
+            unsigned in = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int p = 16 * (j >> 2) + 4 * g + (j & 3);
+                in |= (p >= b0 && p <= b1 ? 1u : 0u) << j;
+            }
+            if (!in) continue;
+            const v4i old = *u;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                unsigned take = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (BITS == 8) take |= (in >> (4 * q + j) & 1 ? 255u : 0u) << (8 * j);
+                    else take |= ((in >> (4 * (q & 1) + j) & 1 ? 15u : 0u) | (in >> (4 * (q & 1) + 8 + j) & 1 ? 240u : 0u)) << (8 * j);
+                w[q] = (int)(((unsigned)w[q] & take) | ((unsigned)old[q] & ~take));
+            }
+        }
+        *u = w;
     }
 }
 
-// a thread a (row, head, dimension)
+// A thread two dimensions of a (row, head), k and v: 16-byte stores (rows stand at 8 bytes' alignment only).  Bound by what it
+// writes, eight bytes or more a digit.
 template <int BITS>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_read(NarrowRows a) {
-    const int stream = blockIdx.z, hd = a.s.heads * a.s.dim;
+    const int stream = blockIdx.z, pairs = (a.s.dim + 1) / 2, hd = a.s.heads * pairs;
     i64 p0, lo, hi;
     narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
-    const i64 n = (hi - lo) * hd;
+    const i64 n = (hi - lo) * hd, half = narrow_half(a.s);
     for (i64 i = (i64)blockIdx.x * NTHREADS + threadIdx.x; i < n; i += (i64)gridDim.x * NTHREADS) {
-        const i64 row = lo + i / hd, p = p0 + row;
-        const int h = (int)(i % hd) / a.s.dim, d = (int)(i % hd) % a.s.dim, b = (int)(p & 63), j = 4 * (b >> 4) + (b & 3), g = (b >> 2) & 3;
+        const int r = (int)(i / hd), w = (int)(i - (i64)r * hd), h = w / pairs, d = 2 * (w - h * pairs);
+        const i64 row = lo + r, p = p0 + row;
+        const int b = (int)(p & 63), j = 4 * (b >> 4) + (b & 3), g = (b >> 2) & 3;
         const char* base = narrow_at(a.buf, a.s, stream, h, (int)(p >> 6));
-        const char* vbase = base + narrow_half(a.s);
-        const unsigned char* lev = reinterpret_cast<const unsigned char*>(vbase + narrow_half(a.s));
-        int kv, vv;
+        const char* vbase = base + half;
+        const unsigned char* lev = reinterpret_cast<const unsigned char*>(vbase + half);
+        const int lk = lev[b], lv = lev[64 + b];
+        int k[2], v[2];
         if (BITS == 8) {
-            kv = (signed char)base[(d >> 4) * 1024 + b * 16 + (d & 15)];
-            vv = (signed char)vbase[(d >> 4) * 1024 + (16 * g + (d & 15)) * 16 + j];
+            const unsigned kb = *reinterpret_cast<const unsigned short*>(base + (d >> 4) * 1024 + b * 16 + (d & 15));
+            k[0] = (signed char)kb; k[1] = (signed char)(kb >> 8);
+#pragma unroll
+            for (int x = 0; x < 2; x++) v[x] = (signed char)vbase[(d >> 4) * 1024 + (16 * g + (d & 15) + x) * 16 + j];
         } else {
-            const int kb = (signed char)base[(d >> 5) * 1024 + b * 16 + (d & 15)];
-            const int vb = (signed char)vbase[(d >> 5) * 1024 + (16 * g + (d & 15)) * 16 + 8 * (d >> 4 & 1) + (j & 7)];
-            kv = d & 16 ? kb >> 4 : (int)((unsigned)kb << 28) >> 28;
-            vv = j & 8 ? vb >> 4 : (int)((unsigned)vb << 28) >> 28;
+            const unsigned kb = *reinterpret_cast<const unsigned short*>(base + (d >> 5) * 1024 + b * 16 + (d & 15)) >> (d & 16 ? 4 : 0);
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const unsigned vb = (unsigned char)vbase[(d >> 5) * 1024 + (16 * g + (d & 15) + x) * 16 + 8 * (d >> 4 & 1) + (j & 7)] >> (j & 8 ? 4 : 0);
+                k[x] = (int)(kb >> (8 * x) << 28) >> 28;
+                v[x] = (int)(vb << 28) >> 28;
+            }
         }
         const i64 at = stream * a.stream_stride + row * a.row_stride + (i64)h * a.s.dim + d;
-        a.k2[at] = shl(kv, lev[b]);
-        a.v2[at] = shl(vv, lev[64 + b]);
+        if (d + 1 < a.s.dim) {
+            *reinterpret_cast<i64x2*>(a.k2 + at) = i64x2{shl(k[0], lk), shl(k[1], lk)};
+            *reinterpret_cast<i64x2*>(a.v2 + at) = i64x2{shl(v[0], lv), shl(v[1], lv)};
+        } else {
+            a.k2[at] = shl(k[0], lk);
+            a.v2[at] = shl(v[0], lv);
+        }
     }
 }
 
@@ -669,9 +704,9 @@ template <int BITS> SMD int narrow_sum(int n0, int n1, int n2) {
 #define SWEEP_ARR 17790            // entries of the arrival that the kernels hold (base2_convert.py:50-53 gives 17,745)
 struct NarrowFactors {
     double h[NARROW_H], l[128];
-    SMD void load(const NarrowAtt& a, int tid) {
+    SMD void load(const NarrowAtt& a, int tid, int threads) {
         const int nh = a.tb.alen / 128 + 1;
-        for (int i = tid; i < nh + 128; i += NTHREADS) (i < nh ? h[i] : l[i - nh]) = a.WF[i];
+        for (int i = tid; i < nh + 128; i += threads) (i < nh ? h[i] : l[i - nh]) = a.WF[i];
     }
     SMD int weight(int d) const {
         const double x = __builtin_fma(h[d >> 7], l[d & 127], 6755399441055746.0);
@@ -826,7 +861,7 @@ template <int DK, int GR>
 SMD void narrow_few(const NarrowAtt& a, int stream, int h, int rt, int lane, int wave, NarrowFew<DK, GR>& f) {
     constexpr int PER = GR * 64 / NTHREADS;                          // a wave's rows: loaded together
     const int rows = min(GR, a.R - rt * GR);
-    f.wf.load(a, wave * 64 + lane);
+    f.wf.load(a, wave * 64 + lane, NTHREADS);
     i64 x[PER][DK];
     int p[PER];
 #pragma unroll
@@ -947,12 +982,13 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
 // B = q, so that a lane holds one row's scores of 16 positions a tile, and exactly the ones, in the order, that its bytes of a
 // weight operand are (the values' layout): nothing moves between lanes.  A first pass over the keys finds each chunk's m_j
 // and E_j (kept in memory) and the row's M and E; the second adds each chunk's N_j f_j in registers, and the waves' sums are
-// added at the end.  Bound by the vector arithmetic of a score, so the arrivals' weights stand in LDS.
+// added at the end.  Bound by the vector arithmetic of a score.
 #define SWEEP_WAVES 4
 template <int BITS, int DK>
-__global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sweep(NarrowAtt a) {
+__global__ __launch_bounds__(64 * SWEEP_WAVES, 4 - (DK == 4 ? 3 : DK)) void k_narrow_sweep(NarrowAtt a) {
     constexpr int DT = 4 * DK, VU = 8 / BITS, NW = SWEEP_WAVES;
-    __shared__ __attribute__((aligned(16))) int tab[SWEEP_ARR + 1];
+    __shared__ i64 sums[NW][DT * 4][64];                             // the waves' N, a lane's own (in registers they spill)
+    __shared__ NarrowFactors wf;
     __shared__ int wm[NW][16], we[NW][16];
     __shared__ i64 wA[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -967,7 +1003,7 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
     phi = __builtin_amdgcn_readfirstlane(phi);
     plo = __builtin_amdgcn_readfirstlane(plo);
     if (phi < 0) return;                                             // (the same in every wave)
-    for (int i = threadIdx.x; i <= a.tb.alen; i += 64 * NW) tab[i] = a.W2[i];
+    wf.load(a, threadIdx.x, 64 * NW);
     v4i q[DK];
     q_operands<BITS, DK>(a.q8 + (head * a.R + rho) * a.s.wide, g, q);
     const i64 half = narrow_half(a.s), tile_bytes = narrow_tile(a.s);
@@ -1045,7 +1081,9 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; w++) { M = max(M, wm[w][n]); E = max(E, we[w][n]); }
-    i64 N[DT][4] = {}, A = 0;
+    i64 A = 0;
+#pragma unroll
+    for (int i = 0; i < DT * 4; i++) sums[wave][i][lane] = 0;
     int have = -1;                                                   // the tile that is loaded
     for (int j = wave; 4 * j <= last; j += NW) {
         // (this wave's own stores, read by the lanes that made them)
@@ -1079,7 +1117,7 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
                             if (64 * T + 16 * sub + 4 * g + r > pos) d = a.tb.alen;
                             sh = max(sh, 0);
                         }
-                        const int u2 = tab[d];
+                        const int u2 = wf.weight(d);
                         Aj += u2;
                         x[r] = narrow_weight(u2, sh);
                     }
@@ -1109,41 +1147,26 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, DK == 4 ? 1 : 2) void k_narrow_sw
 #pragma unroll
         for (int c = 0; c < DT; c++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) N[c][r] += rsh_round((i64)narrow_sum<BITS>(C[0][c][r], C[1][c][r], C[2][c][r]) * f, sh);
+            for (int r = 0; r < 4; r++) sums[wave][4 * c + r][lane] += rsh_round((i64)narrow_sum<BITS>(C[0][c][r], C[1][c][r], C[2][c][r]) * f, sh);
     }
-    // the waves' sums through the table's place, half of a wave's a time where they are many; wave w finishes every fourth
-    // dimension tile
-    __syncthreads();
+    // the waves' sums added: wave w finishes every fourth dimension tile
     if (g == 0) wA[wave][n] = A;
-    i64* part = reinterpret_cast<i64*>(tab);                         // [NW][DT / HALVES][4][64]
-    constexpr int HALVES = DK == 4 ? 2 : 1, DH = DT / HALVES;
-    static_assert(NW * DH * 4 * 64 * 8 <= sizeof(tab), "the waves' sums fit the table's place");
+    __syncthreads();
+    if (pos < 0 || rt * 16 + n >= a.R) return;
+    A = 0;
+    for (int w = 0; w < NW; w++) A += wA[w][n];
+    const i64 F = ((i64)E + 8) * 65536 - log2fix(A, a.tb);
     const int tt = rho / a.group, hq = h * a.group + rho % a.group;
     i64* o = a.out + stream * a.o_stream + tt * a.o_row + (i64)hq * a.s.dim;
+    for (int c = wave; c < DT; c += NW)
 #pragma unroll
-    for (int hf = 0; hf < HALVES; hf++) {
+        for (int r = 0; r < 4; r++) {
+            i64 s = 0;
 #pragma unroll
-        for (int c = 0; c < DH; c++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) part[((wave * DH + c) * 4 + r) * 64 + lane] = N[hf * DH + c][r];
-        __syncthreads();
-        if (hf == 0) {
-            A = 0;
-            for (int w = 0; w < NW; w++) A += wA[w][n];
+            for (int w = 0; w < NW; w++) s += sums[w][4 * c + r][lane];
+            const int d = 16 * c + 4 * g + r;
+            if (d < a.s.dim) o[d] = power(s, F, a.tb);
         }
-        const i64 F = ((i64)E + 8) * 65536 - log2fix(A, a.tb);
-        if (pos >= 0 && rt * 16 + n < a.R)
-            for (int c = wave; c < DH; c += NW)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    i64 s = 0;
-#pragma unroll
-                    for (int w = 0; w < NW; w++) s += part[((w * DH + c) * 4 + r) * 64 + lane];
-                    const int d = 16 * (hf * DH + c) + 4 * g + r;
-                    if (d < a.s.dim) o[d] = power(s, F, a.tb);
-                }
-        __syncthreads();
-    }
 }
 
 // A block a row: its chunks joined.  The chunks' factors and shifts are formed once, in LDS, a batch of NT chunks at a
@@ -1380,7 +1403,7 @@ extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, i
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_read: the cache is not in a device's memory");
     a.buf = static_cast<char*>(const_cast<void*>(buf)); a.k2 = (i64*)k; a.v2 = (i64*)v;
     a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
-    const i64 n = (i64)rows * a.s.heads * a.s.dim;
+    const i64 n = (i64)rows * a.s.heads * ((a.s.dim + 1) / 2);
     const dim3 grid((unsigned)std::min<i64>((n + NTHREADS - 1) / NTHREADS, 4096), 1, (unsigned)a.s.streams);
     if (a.s.bits == 4) launch(g_kt.stages, "narrow.read", k_narrow_read<4>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
     else launch(g_kt.stages, "narrow.read", k_narrow_read<8>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
