@@ -9,6 +9,20 @@
 // l % 16, bytes k = 16 (l / 16) + b), so an operand is one 16-byte load a lane, no lane's bytes are moved between lanes
 // and a wave's loads are 1 KB in a row.
 #define NTHREADS 256
+// Results of NARROW_STREAM bytes and more are stored past the caches (nontemporal): left in the 256 MB behind them, a large
+// result is written out while the next kernel reads, which then takes half as long again (three prompts of 2,048 rows
+// written and read back 37 against 50 us, 4,096 rows 4,096 -> 11,008 249 against 270 us).  Smaller ones stay cached for
+// whoever reads them (64 rows 768 -> 50,257 18.2 us stored past the caches, 17.2 not).
+#define NARROW_STREAM (64 << 20)
+typedef i64 i64x2 __attribute__((ext_vector_type(2), aligned(8)));       // (rows stand at 8 bytes' alignment only)
+template <bool NT> SMD void put(i64* p, i64 v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+template <bool NT> SMD void put2(i64* p, i64 v, i64 w) {
+    if constexpr (NT) __builtin_nontemporal_store(i64x2{v, w}, reinterpret_cast<i64x2*>(p));
+    else *reinterpret_cast<i64x2*>(p) = i64x2{v, w};
+}
 
 // x 2^-s rounded half up without the sum that wraps near 2^63 (s in 0 .. 63)
 SMD i64 rsh_round(i64 x, int s) { return s > 0 ? (x >> s) + ((x >> (s - 1)) & 1) : x; }
@@ -55,8 +69,7 @@ SMD unsigned digit_quad(const i64 v[4], int sh) {
     }
     return w;
 }
-// four values of a row from place 4 q, zeros past its end (rows stand at 8 bytes' alignment only)
-typedef i64 i64x2 __attribute__((ext_vector_type(2), aligned(8)));
+// four values of a row from place 4 q, zeros past its end
 SMD void row_quad(const i64* x, int q, int nin, i64 v[4]) {
     if (4 * q + 3 < nin) {
         const i64x2 lo = *reinterpret_cast<const i64x2*>(x + 4 * q), hi = *reinterpret_cast<const i64x2*>(x + 4 * q + 2);
@@ -66,34 +79,35 @@ SMD void row_quad(const i64* x, int q, int nin, i64 v[4]) {
         for (int i = 0; i < 4; i++) v[i] = 4 * q + i < nin ? x[4 * q + i] : 0;
     }
 }
-// one block a row: the row's level, then its digits in the operand's order (four in a row a thread).  Rows of up to
-// 8,192 values are held in registers between the two passes, longer ones are read again.  Bound by the rows' read.  The 16
-// rows of a tile share their 128-byte lines of digits: with many rows, blocks of one die (every eighth) take one tile, so
-// that the lines fill in that die's L2.
+// two values of a row from place i, zeros past its end
+SMD i64x2 row_pair(const i64* x, int i, int nin) {
+    if (i + 1 < nin) return *reinterpret_cast<const i64x2*>(x + i);
+    return i64x2{i < nin ? x[i] : 0, 0};
+}
+// One block a row: the row's level, then its digits in the operand's order.  A thread loads two values in a row, so that a
+// wave's load is 1 KB in a row (16 bytes every 32, four values a thread, touch each line twice: 53 us at 4096 rows of 4096),
+// and pairs of threads swap halves to store four digits each.  Rows of up to 8,192 values are held in registers between the
+// two passes, longer ones are read again.  Bound by the rows' read.  The 16 rows of a tile share their 128-byte lines of
+// digits: with many rows, blocks of one die (every eighth) take one tile, so that the lines fill in that die's L2.
 __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
-    constexpr int HOLD = 8;
+    constexpr int HOLD = 8, STEP = 4 * NTHREADS;
     __shared__ u64 wor[NTHREADS / 64];
     const int b = blockIdx.x, r = gridDim.x >= 128 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
-    const int tid = threadIdx.x, quads = a.K / 4;
+    const int tid = threadIdx.x;
     if (r >= a.rows) return;
     const i64* x = a.X + (i64)r * a.ldx;
-    i64 held[HOLD][4];
+    struct Four { i64x2 lo, hi; };                                   // places i + 2 tid and i + STEP / 2 + 2 tid
+    auto load = [&](int i) { return Four{row_pair(x, i + 2 * tid, a.nin), row_pair(x, i + STEP / 2 + 2 * tid, a.nin)}; };
+    auto mags = [](const Four& f) { return mag64(f.lo[0]) | mag64(f.lo[1]) | mag64(f.hi[0]) | mag64(f.hi[1]); };
+    Four held[HOLD];
     u64 orr = 0;
 #pragma unroll
-    for (int s = 0; s < HOLD; s++) {
-        const int q = tid + s * NTHREADS;
-        if (q < quads) {
-            row_quad(x, q, a.nin, held[s]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) orr |= mag64(held[s][i]);
+    for (int s = 0; s < HOLD; s++)
+        if (s * STEP < a.K) {
+            held[s] = load(s * STEP);
+            orr |= mags(held[s]);
         }
-    }
-    for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
-        i64 v[4];
-        row_quad(x, q, a.nin, v);
-#pragma unroll
-        for (int i = 0; i < 4; i++) orr |= mag64(v[i]);
-    }
+    for (int i = HOLD * STEP; i < a.K; i += STEP) orr |= mags(load(i));
     orr = wave_or_u64(orr);
     if ((tid & 63) == 0) wor[tid >> 6] = orr;
     __syncthreads();
@@ -103,18 +117,19 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
     const int sh = digit_level(orr, 8);
     if (tid == 0) a.level[r] = sh;
     signed char* o = a.lights + (i64)(r >> 4) * a.K * 16 + (r & 15) * 16;
-    auto store = [&](int q, const i64 v[4]) {
-        const int k = 4 * q;
-        *reinterpret_cast<unsigned*>(o + (i64)(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 15)) = digit_quad(v, sh);
+    const bool odd = tid & 1;
+    auto store = [&](int i, const Four& f) {
+        const i64 v[4] = {f.lo[0], f.lo[1], f.hi[0], f.hi[1]};
+        const unsigned d = digit_quad(v, sh);                        // low half: the first place's two
+        const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)d, 0xB1, 0xf, 0xf, false);      // the thread beside
+        const unsigned w = odd ? (other >> 16) | (d & 0xFFFF0000u) : (d & 0xFFFFu) | (other << 16);
+        const int k = i + (odd ? STEP / 2 + 2 * tid - 2 : 2 * tid);
+        if (k < a.K) *reinterpret_cast<unsigned*>(o + (i64)(k >> 6) * 1024 + ((k >> 4) & 3) * 256 + (k & 15)) = w;
     };
 #pragma unroll
     for (int s = 0; s < HOLD; s++)
-        if (tid + s * NTHREADS < quads) store(tid + s * NTHREADS, held[s]);
-    for (int q = tid + HOLD * NTHREADS; q < quads; q += NTHREADS) {
-        i64 v[4];
-        row_quad(x, q, a.nin, v);
-        store(q, v);
-    }
+        if (s * STEP < a.K) store(s * STEP, held[s]);
+    for (int i = HOLD * STEP; i < a.K; i += STEP) store(i, load(i));
 }
 
 SMD v4i mfma8(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
@@ -246,7 +261,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
 // reads rearrange anything and no two lanes meet in a bank), ST - 1 stages ahead.
 typedef const __attribute__((address_space(1))) void* gas_p;
 typedef __attribute__((address_space(3))) void* las_p;
-template <int WR, int WC, int RT, int CT>
+template <int WR, int WC, int RT, int CT, bool NT>
 __global__ __launch_bounds__(64 * WR * WC, 2) void k_narrow_tiles(Narrow8Args a, int tr, int tc) {
     constexpr int W = WR * WC, AF = WR * RT, F = AF + WC * CT, LPW = F / W;
     static_assert(F % W == 0, "every wave loads the same number of fragments");
@@ -330,7 +345,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void k_narrow_tiles(Narrow8Args a,
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int row = (br * AF + wr * RT + r) * 16 + 4 * g + i;
-                if (row < a.rows) a.out[(i64)row * a.ldo + col] = narrow_out(acc[r][c][i], we, lev[r][i], wb);
+                if (row < a.rows) put<NT>(&a.out[(i64)row * a.ldo + col], narrow_out(acc[r][c][i], we, lev[r][i], wb));
             }
     }
 }
@@ -390,12 +405,13 @@ template <int BITS, int WIDE>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
     constexpr int PER = WIDE / 64, AT_ONCE = PER == 4 ? 2 : 4, NW = NTHREADS / 64;
     __shared__ __attribute__((aligned(16))) signed char kd[64][WIDE + 4], vd[WIDE][68];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, stream = blockIdx.z;
+    // (the heads first: blocks that run together read whole rows)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x % a.s.heads, stream = blockIdx.z;
     i64 p0, lo, hi;
     narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
     if (lo >= hi) return;
     const i64 first = p0 + lo, last = p0 + hi - 1;                // positions written
-    const i64 tile = first / 64 + blockIdx.x;
+    const i64 tile = first / 64 + blockIdx.x / a.s.heads;
     if (tile > last / 64) return;
     const int b0 = (int)max(first - tile * 64, (i64)0), b1 = (int)min(last - tile * 64, (i64)63);    // within the tile
     char* base = narrow_at(a.buf, a.s, stream, head, (int)tile);
@@ -483,14 +499,14 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
 
 // A thread two dimensions of a (row, head), k and v: 16-byte stores (rows stand at 8 bytes' alignment only).  Bound by what it
 // writes, eight bytes or more a digit.
-template <int BITS>
+template <int BITS, bool NT>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_read(NarrowRows a) {
     const int stream = blockIdx.z, pairs = (a.s.dim + 1) / 2, hd = a.s.heads * pairs;
     i64 p0, lo, hi;
     narrow_range(a.start, a.count, stream, a.rows, a.s.ctx, p0, lo, hi);
     const i64 n = (hi - lo) * hd, half = narrow_half(a.s);
     for (i64 i = (i64)blockIdx.x * NTHREADS + threadIdx.x; i < n; i += (i64)gridDim.x * NTHREADS) {
-        const int r = (int)(i / hd), w = (int)(i - (i64)r * hd), h = w / pairs, d = 2 * (w - h * pairs);
+        const int r = n <= UINT_MAX ? (int)((unsigned)i / (unsigned)hd) : (int)(i / hd), w = (int)(i - (i64)r * hd), h = w / pairs, d = 2 * (w - h * pairs);
         const i64 row = lo + r, p = p0 + row;
         const int b = (int)(p & 63), j = 4 * (b >> 4) + (b & 3), g = (b >> 2) & 3;
         const char* base = narrow_at(a.buf, a.s, stream, h, (int)(p >> 6));
@@ -514,8 +530,8 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_read(NarrowRows a) {
         }
         const i64 at = stream * a.stream_stride + row * a.row_stride + (i64)h * a.s.dim + d;
         if (d + 1 < a.s.dim) {
-            *reinterpret_cast<i64x2*>(a.k2 + at) = i64x2{shl(k[0], lk), shl(k[1], lk)};
-            *reinterpret_cast<i64x2*>(a.v2 + at) = i64x2{shl(v[0], lv), shl(v[1], lv)};
+            put2<NT>(a.k2 + at, shl(k[0], lk), shl(k[1], lk));
+            put2<NT>(a.v2 + at, shl(v[0], lv), shl(v[1], lv));
         } else {
             a.k2[at] = shl(k[0], lk);
             a.v2[at] = shl(v[0], lv);
@@ -713,6 +729,11 @@ struct NarrowFactors {
         return (int)((unsigned)__builtin_bit_cast(u64, x) >> 1 & ~1u);
     }
 };
+
+// A chunk's N_j f_j rounded by s >= 24 places, added in float64: |N_j| is at most 2^29 and f_j at most 2^24, so the product, its
+// half and the sum of up to 2^16 chunks are exact (and a quarter of the steps of 64-bit whole numbers)
+SMD double narrow_factor(int f, int s) { return ldexp((double)f, -s); }
+SMD double narrow_joined(double N, int Nj, double f) { return N + floor(__builtin_fma((double)Nj, f, 0.5)); }
 
 // Few rows: a wave a chunk, a tile of GR rows (RU of every four wanted).  Scores: A = q, B = keys, so a lane is a position.
 // With fewer than 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position
@@ -987,7 +1008,7 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
 template <int BITS, int DK>
 __global__ __launch_bounds__(64 * SWEEP_WAVES, 4 - (DK == 4 ? 3 : DK)) void k_narrow_sweep(NarrowAtt a) {
     constexpr int DT = 4 * DK, VU = 8 / BITS, NW = SWEEP_WAVES;
-    __shared__ i64 sums[NW][DT * 4][64];                             // the waves' N, a lane's own (in registers they spill)
+    __shared__ double sums[NW][DT * 4][64];                             // the waves' N, a lane's own (in registers they spill)
     __shared__ NarrowFactors wf;
     __shared__ int wm[NW][16], we[NW][16];
     __shared__ i64 wA[NW][16];
@@ -1143,11 +1164,14 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, 4 - (DK == 4 ? 3 : DK)) void k_na
         Aj += __shfl_xor(Aj, 16, 64);
         Aj += __shfl_xor(Aj, 32, 64);
         A += rsh_round((i64)(Aj >> 1) * f, 24);                      // (Aj 2^31 at most)
-        const int sh = min(24 + E - e, 63);
+        const double fs = narrow_factor(f, 24 + E - e);
 #pragma unroll
         for (int c = 0; c < DT; c++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) sums[wave][4 * c + r][lane] += rsh_round((i64)narrow_sum<BITS>(C[0][c][r], C[1][c][r], C[2][c][r]) * f, sh);
+            for (int r = 0; r < 4; r++) {
+                double& N = sums[wave][4 * c + r][lane];
+                N = narrow_joined(N, narrow_sum<BITS>(C[0][c][r], C[1][c][r], C[2][c][r]), fs);
+            }
     }
     // the waves' sums added: wave w finishes every fourth dimension tile
     if (g == 0) wA[wave][n] = A;
@@ -1161,70 +1185,77 @@ __global__ __launch_bounds__(64 * SWEEP_WAVES, 4 - (DK == 4 ? 3 : DK)) void k_na
     for (int c = wave; c < DT; c += NW)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            i64 s = 0;
+            double s = 0;
 #pragma unroll
             for (int w = 0; w < NW; w++) s += sums[w][4 * c + r][lane];
             const int d = 16 * c + 4 * g + r;
-            if (d < a.s.dim) o[d] = power(s, F, a.tb);
+            if (d < a.s.dim) o[d] = power((i64)s, F, a.tb);
         }
 }
 
-// A block a row: its chunks joined.  The chunks' factors and shifts are formed once, in LDS, a batch of NT chunks at a
-// time; then NT / wide slices of chunks, a thread a dimension, eight loads in flight.
-template <int NT>
-__global__ __launch_bounds__(NT) void k_narrow_join(NarrowAtt a) {
-    __shared__ int sm[NT / 64], se[NT / 64], sf[NT], ss[NT];
-    __shared__ i64 sa[NT / 64], sn[NT];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rho = blockIdx.x, h = blockIdx.y, stream = blockIdx.z;
+// A block a row's db dimensions: its chunks joined, a thread a dimension of a slice of the chunks (NTHREADS / db slices).  The
+// first PRE sums of a thread are loaded with all else, before the row's M and E are known; the chunks' factors are formed
+// once, in LDS, a batch of NTHREADS chunks at a time.  Bound by its chain of loads with few chunks (all of a row's dimensions
+// in one block then: the factors are formed once), by their number with many (8 dimensions a block: 512 chunks of 32 rows 12.0 us, 15.0 with 16 a block, 25.3 with 32).
+__global__ __launch_bounds__(NTHREADS, 8) void k_narrow_join(NarrowAtt a, int db) {
+    constexpr int PRE = 8, NW = NTHREADS / 64;
+    __shared__ int sm[NW], se[NW];
+    __shared__ i64 sa[NW];
+    __shared__ double sf[NTHREADS], sn[NTHREADS];
+    const int wide = a.s.wide, blocks = wide / db;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rho = blockIdx.x / blocks, h = blockIdx.y, stream = blockIdx.z;
     const i64 head = (i64)stream * a.s.heads + h, slot0 = head * a.J * a.R + rho;
     const int p = narrow_pos(a, stream, rho / a.group);
     if (p < 0) return;
-    const int J = p / NCHUNK + 1;
+    const int J = p / NCHUNK + 1, d = (int)blockIdx.x % blocks * db + tid % db, slice = tid / db, slices = NTHREADS / db;
+    const int* pn = a.pN + slot0 * wide + d;
+    const i64 step = (i64)a.R * wide;
+    int v[PRE];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < PRE; i++)
+            if (j0 + i * slices < J) v[i] = pn[(j0 + i * slices) * step];
+    };
+    load(slice);
     int M = NARROW_NONE, E = 0;
-    for (int j = tid; j < J; j += NT) {
+    for (int j = tid; j < J; j += NTHREADS) {
         M = max(M, a.pm[slot0 + (i64)j * a.R]);
         E = max(E, a.pE[slot0 + (i64)j * a.R]);
     }
     for (int o = 1; o < 64; o <<= 1) { M = max(M, __shfl_xor(M, o, 64)); E = max(E, __shfl_xor(E, o, 64)); }
     if (lane == 0) { sm[wave] = M; se[wave] = E; }
     __syncthreads();
-    for (int i = 0; i < NT / 64; i++) { M = max(M, sm[i]); E = max(E, se[i]); }
-    const int wide = a.s.wide, d = tid % wide, slice = tid / wide, slices = NT / wide;
-    i64 A = 0, N = 0;
-    for (int j0 = 0; j0 < J; j0 += NT) {
-        const int n = min(NT, J - j0);
-        __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; i++) { M = max(M, sm[i]); E = max(E, se[i]); }
+    i64 A = 0;
+    double N = 0;
+    for (int j0 = 0; j0 < J; j0 += NTHREADS) {
+        const int n = min(NTHREADS, J - j0);
+        if (j0) __syncthreads();
         if (tid < n) {
             const i64 s = slot0 + (i64)(j0 + tid) * a.R;
             const unsigned df = (unsigned)M - (unsigned)a.pm[s];
             const int f = df < (unsigned)a.tb.alen ? a.tb.ARR[df] : 0;
             A += rsh_round((i64)a.pA[s] * f, 24);
-            sf[tid] = f;
-            ss[tid] = min(24 + E - a.pE[s], 63);
+            sf[tid] = narrow_factor(f, 24 + E - a.pE[s]);
         }
         __syncthreads();
-        const int* pn = a.pN + (slot0 + (i64)j0 * a.R) * wide + d;
-        const i64 step = (i64)a.R * wide;
-        int j = slice;
-        for (; j + 7 * slices < n; j += 8 * slices) {
-            int v[8];
+        for (int j = slice; j < n; j += PRE * slices) {
+            if (j0 + j != slice) load(j0 + j);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = pn[(j + i * slices) * step];
-#pragma unroll
-            for (int i = 0; i < 8; i++) N += rsh_round((i64)v[i] * sf[j + i * slices], ss[j + i * slices]);
+            for (int i = 0; i < PRE; i++)
+                if (j + i * slices < n) N = narrow_joined(N, v[i], sf[j + i * slices]);
         }
-        for (; j < n; j += slices) N += rsh_round((i64)pn[j * step] * sf[j], ss[j]);
     }
     A = wave_reduce64(A, OpAdd());
     if (lane == 0) sa[wave] = A;
     sn[tid] = N;
     __syncthreads();
-    if (tid >= a.s.dim) return;
-    A = 0;
-    for (int i = 0; i < NT / 64; i++) A += sa[i];
-    for (int i = 1; i < slices; i++) N += sn[i * wide + d];
+    if (tid >= db || d >= a.s.dim) return;
+    A = sa[0] + sa[1] + sa[2] + sa[3];
+    for (int i = 1; i < slices; i++) N += sn[i * db + tid];
     const int t = rho / a.group, hq = h * a.group + rho % a.group;
-    a.out[stream * a.o_stream + t * a.o_row + (i64)hq * a.s.dim + d] = power(N, ((i64)E + 8) * 65536 - log2fix(A, a.tb), a.tb);
+    a.out[stream * a.o_stream + t * a.o_row + (i64)hq * a.s.dim + d] = power((i64)N, ((i64)E + 8) * 65536 - log2fix(A, a.tb), a.tb);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -1331,14 +1362,16 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     const int nt = (a.N + 15) / 16, rts = (rows + 15) / 16;
     if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
     else if (rts == 2) launch(g_kt.stages, "plate8.rows", k_narrow_rows<2, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
-    else if (rows <= 256) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3(nt, (rts + 3) / 4), dim3(NTHREADS), 0, s, a);
+    else if (rows <= 256) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 1>, dim3((unsigned)(nt + 3) / 4, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
     else {
         auto tiles = [&](auto kern, int rt, int ct, int threads) {
             const int tr = (rts + rt - 1) / rt, tc = (nt + ct - 1) / ct;
             launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)((tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
         };
-        if ((i64)((rts + 15) / 16) * ((nt + 15) / 16) >= 192) tiles(k_narrow_tiles<2, 4, 8, 4>, 16, 16, 512);
-        else tiles(k_narrow_tiles<2, 2, 4, 4>, 8, 8, 256);
+        // (256 x 256 tiles from three quarters of a tile a CU on; they are then too large for a result that stays cached)
+        if ((i64)((rts + 15) / 16) * ((nt + 15) / 16) >= 192) tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512);
+        else if ((i64)rows * a.N * 8 >= NARROW_STREAM) tiles(k_narrow_tiles<2, 2, 4, 4, true>, 8, 8, 256);
+        else tiles(k_narrow_tiles<2, 2, 4, 4, false>, 8, 8, 256);
     }
     HIP_TRY(hipGetLastError());
     return SM_OK;
@@ -1386,7 +1419,9 @@ extern "C" int sm_narrow_write(const sm_narrow* c, void* buf, const int64_t* k, 
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_write: the cache is not in a device's memory");
     a.buf = static_cast<char*>(buf); a.k = (const i64*)k; a.v = (const i64*)v;
     a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
-    const dim3 grid((unsigned)((rows + 62) / 64 + 1), (unsigned)a.s.heads, (unsigned)a.s.streams);
+    const i64 blocks = (i64)((rows + 62) / 64 + 1) * a.s.heads;
+    if (blocks > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_write: too many rows for one call");
+    const dim3 grid((unsigned)blocks, 1, (unsigned)a.s.streams);
     auto go = [&](auto kern) { launch(g_kt.stages, "narrow.write", kern, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a); };
     if (a.s.bits == 4) a.s.wide == 64 ? go(k_narrow_write<4, 64>) : a.s.wide == 128 ? go(k_narrow_write<4, 128>) : go(k_narrow_write<4, 256>);
     else a.s.wide == 64 ? go(k_narrow_write<8, 64>) : a.s.wide == 128 ? go(k_narrow_write<8, 128>) : go(k_narrow_write<8, 256>);
@@ -1405,8 +1440,10 @@ extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, i
     a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
     const i64 n = (i64)rows * a.s.heads * ((a.s.dim + 1) / 2);
     const dim3 grid((unsigned)std::min<i64>((n + NTHREADS - 1) / NTHREADS, 4096), 1, (unsigned)a.s.streams);
-    if (a.s.bits == 4) launch(g_kt.stages, "narrow.read", k_narrow_read<4>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
-    else launch(g_kt.stages, "narrow.read", k_narrow_read<8>, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a);
+    auto go = [&](auto kern) { launch(g_kt.stages, "narrow.read", kern, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a); };
+    const bool nt = (i64)a.s.streams * rows * a.s.heads * a.s.dim * 16 >= NARROW_STREAM;
+    if (a.s.bits == 4) nt ? go(k_narrow_read<4, true>) : go(k_narrow_read<4, false>);
+    else nt ? go(k_narrow_read<8, true>) : go(k_narrow_read<8, false>);
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
@@ -1465,9 +1502,8 @@ static void narrow_attend(const NarrowAtt& a, bool sweep, hipStream_t st) {
     else if (gr == 4) split(k_narrow_split<BITS, DK, 4, 4>);
     else if (gr == 8) split(k_narrow_split<BITS, DK, 8, 4>);
     else split(k_narrow_split<BITS, DK, 16, 4>);
-    const dim3 rgrid((unsigned)a.R, heads, streams);
-    if (a.J > 32) launch(g_kt.stages, "narrow.join", k_narrow_join<1024>, rgrid, dim3(1024), 0, st, a);
-    else launch(g_kt.stages, "narrow.join", k_narrow_join<256>, rgrid, dim3(256), 0, st, a);
+    const int db = a.J > 64 ? 8 : a.s.wide;
+    launch(g_kt.stages, "narrow.join", k_narrow_join, dim3((unsigned)(a.R * (a.s.wide / db)), heads, streams), dim3(NTHREADS), 0, st, a, db);
 }
 
 extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const void* buf, const int64_t* q, int64_t q_row, int64_t q_stream,
