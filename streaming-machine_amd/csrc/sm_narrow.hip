@@ -878,22 +878,22 @@ SMD bool narrow_reach(const NarrowAtt& a, int stream, int first, int end, int& p
     phi = (int)min(s0 + tz, (i64)a.span - 1);
     return tz >= ta && phi >= 0;
 }
-template <int DK, int GR>
+template <int NW, int DK, int GR>
 SMD void narrow_few(const NarrowAtt& a, int stream, int h, int rt, int lane, int wave, NarrowFew<DK, GR>& f) {
-    constexpr int PER = GR * 64 / NTHREADS;                          // a wave's rows: loaded together
+    constexpr int PER = (GR + NW - 1) / NW;                          // a wave's rows: loaded together
     const int rows = min(GR, a.R - rt * GR);
-    f.wf.load(a, wave * 64 + lane, NTHREADS);
+    f.wf.load(a, wave * 64 + lane, 64 * NW);
     i64 x[PER][DK];
     int p[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        const int r = wave + i * (NTHREADS / 64), rho = rt * GR + r, t = rho / a.group;
+        const int r = wave + i * NW, rho = rt * GR + r, t = rho / a.group;
         p[i] = r < rows ? narrow_pos(a, stream, t) : -1;
         narrow_q_load<DK>(a, a.q + stream * a.q_stream + t * a.q_row + ((i64)h * a.group + rho % a.group) * a.s.dim, p[i] >= 0, lane, x[i]);
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-        const int r = wave + i * (NTHREADS / 64);
+        const int r = wave + i * NW;
         if (r >= rows) break;
         const int e = narrow_q_row<DK>(a, x[i], lane, f.qd[r]);
         if (lane == 0) { f.qe[r] = e; f.qp[r] = p[i]; }
@@ -914,7 +914,7 @@ SMD void narrow_ready(NarrowChunk<BITS, DK, GR, RU>& c, const NarrowFew<DK, GR>&
 
 // a block: NTHREADS / 64 chunks of one row tile, their partial sums to memory (k_narrow_join)
 template <int BITS, int DK, int GR, int RU>
-__global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow_split(NarrowAtt a, int jblocks) {
+__global__ __launch_bounds__(NTHREADS, DK <= 2 ? 2 : 1) void k_narrow_split(NarrowAtt a, int jblocks) {
     using Chunk = NarrowChunk<BITS, DK, GR, RU>;
     __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
     __shared__ __attribute__((aligned(16))) NarrowFew<DK, GR> few;
@@ -925,7 +925,7 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
     const i64 head = (i64)stream * a.s.heads + h;
     int plo, phi;
     if (!narrow_reach(a, stream, rt * GR, min(rt * GR + GR, a.R), plo, phi) || phi < jb * (NTHREADS / 64) * NCHUNK) return;
-    narrow_few<DK, GR>(a, stream, h, rt, lane, wave, few);
+    narrow_few<NTHREADS / 64, DK, GR>(a, stream, h, rt, lane, wave, few);
     if (j >= a.J || c0 > phi) return;
     Chunk c;
     narrow_ready(c, few, rows, lane);
@@ -946,23 +946,21 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
         }
 }
 
-// The same where a block takes all the chunks of its row tile (J <= NEAR): their partial sums stay in LDS and are joined there
-#define NARROW_NEAR 4
-template <int BITS, int DK, int GR, int RU>
-__global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow_near(NarrowAtt a) {
+// The same where a block takes all the chunks of its row tile (J <= NW): their partial sums stay in LDS and are joined there
+template <int BITS, int DK, int GR, int RU, int NW>
+__global__ __launch_bounds__(64 * NW, DK <= 2 ? 2 : 1) void k_narrow_near(NarrowAtt a) {
     using Chunk = NarrowChunk<BITS, DK, GR, RU>;
     constexpr int WIDE = 64 * DK;
-    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NTHREADS / 64][Chunk::WBUF];
+    __shared__ __attribute__((aligned(16))) unsigned char wbuf[NW][Chunk::WBUF];
     __shared__ __attribute__((aligned(16))) NarrowFew<DK, GR> few;
-    __shared__ int pN[NARROW_NEAR][GR][WIDE], pm[NARROW_NEAR][GR], pA[NARROW_NEAR][GR], pE[NARROW_NEAR][GR];
+    __shared__ int pN[NW][GR][WIDE], pm[NW][GR], pA[NW][GR], pE[NW][GR];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int rt = blockIdx.x, h = blockIdx.y, stream = blockIdx.z, rows = a.R - rt * GR;
     const i64 head = (i64)stream * a.s.heads + h;
     int plo, phi;
     if (!narrow_reach(a, stream, rt * GR, min(rt * GR + GR, a.R), plo, phi)) return;
-    narrow_few<DK, GR>(a, stream, h, rt, lane, wave, few);
+    narrow_few<NW, DK, GR>(a, stream, h, rt, lane, wave, few);
     static_assert((SWEEP_ARR + 1) / 128 + 1 <= NARROW_H, "the arrival's factors fit");
-    static_assert(NARROW_NEAR == NTHREADS / 64, "a wave a chunk");
     const int c0 = wave * NCHUNK;
     if (c0 <= phi) {
         Chunk c;
@@ -982,7 +980,7 @@ __global__ __launch_bounds__(NTHREADS, GR == 4 && DK <= 2 ? 2 : 1) void k_narrow
             }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < min(GR, rows) * WIDE; i += NTHREADS) {
+    for (int i = threadIdx.x; i < min(GR, rows) * WIDE; i += 64 * NW) {
         const int r = i / WIDE, d = i % WIDE, p = few.qp[r], J = p / NCHUNK + 1;
         if (p < 0 || d >= a.s.dim) continue;
         int M = pm[0][r], E = pE[0][r];
@@ -1488,12 +1486,21 @@ static void narrow_attend(const NarrowAtt& a, bool sweep, hipStream_t st) {
         return;
     }
     const int gr = a.R <= 4 ? 4 : a.R <= 8 ? 8 : 16, rts = (a.R + gr - 1) / gr, jb = (a.J + NTHREADS / 64 - 1) / (NTHREADS / 64);
-    if (a.J <= NARROW_NEAR) {
-        auto near = [&](auto kern) { launch(g_kt.stages, "narrow.near", kern, dim3((unsigned)rts, heads, streams), dim3(NTHREADS), 0, st, a); };
-        if (a.R == 1) near(k_narrow_near<BITS, DK, 4, 1>);
-        else if (gr == 4) near(k_narrow_near<BITS, DK, 4, 4>);
-        else if (gr == 8) near(k_narrow_near<BITS, DK, 8, 4>);
-        else near(k_narrow_near<BITS, DK, 16, 4>);
+    // one launch where a block's waves hold all the chunks (one stream at 500 positions 9.1 us a call, 11.7 in two launches); of
+    // eight chunks only with four rows a tile (the wider ones' work then stands in too few blocks: 15 rows of 5 heads, nine
+    // streams at 1,733 positions, 26.5 us against 16.2 + 5.1)
+    const dim3 tiles((unsigned)rts, heads, streams);
+    auto near = [&](auto kern, int waves) { launch(g_kt.stages, "narrow.near", kern, tiles, dim3((unsigned)(64 * waves)), 0, st, a); };
+    if (a.J <= 4) {
+        if (a.R == 1) near(k_narrow_near<BITS, DK, 4, 1, 4>, 4);
+        else if (gr == 4) near(k_narrow_near<BITS, DK, 4, 4, 4>, 4);
+        else if (gr == 8) near(k_narrow_near<BITS, DK, 8, 4, 4>, 4);
+        else near(k_narrow_near<BITS, DK, 16, 4, 4>, 4);
+        return;
+    }
+    if (a.J <= 8 && gr == 4) {
+        if (a.R == 1) near(k_narrow_near<BITS, DK, 4, 1, 8>, 8);
+        else near(k_narrow_near<BITS, DK, 4, 4, 8>, 8);
         return;
     }
     const dim3 grid((unsigned)(jb * rts), heads, streams);

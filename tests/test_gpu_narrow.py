@@ -239,6 +239,35 @@ def test_lengths(sm, dtabs, tabs, n):
         attend(c, o, buf, dtabs, tabs, shape, rng, 2, 1, [n - 1], None, 513)
 
 
+@pytest.mark.parametrize("bits,dim,group,ctx", [(4, 64, 1, 1025), (8, 64, 4, 1300), (4, 128, 1, 2048), (8, 128, 3, 1537), (4, 256, 2, 1100),
+                                                (8, 256, 1, 1281), (4, 64, 6, 1100), (8, 128, 16, 1030), (4, 64, 1, 2049), (4, 128, 2, 2300)])
+def test_longer_contexts(sm, dtabs, tabs, bits, dim, group, ctx):
+    """five chunks and more: in one block's waves, and split and joined"""
+    shape = (2, 1, dim, ctx, bits)
+    rng = np.random.default_rng(ctx)
+    c, o, buf = filled_by_columns(sm, rng, shape)
+    attend(c, o, buf, dtabs, tabs, shape, rng, group, 1, [ctx - 1, 900], None, ctx)
+
+
+def test_long_context(sm, dtabs, tabs):
+    """more chunks than the join's block has threads: 70,000 positions, the other stream's row near its start"""
+    shape = (2, 1, 64, 70000, 4)
+    rng = np.random.default_rng(70)
+    c, o = sm.NarrowCache(*shape), orc.Cache(*shape)
+    k, v = (rows_of(rng, (2, 500, 1, 64), 12, 20) for _ in range(2))
+    o.write(k, v, [0, 0])
+    for name in ("k", "v", "kl", "vl"):                  # the same 500 rows over and over
+        a = getattr(o, name)
+        for p in range(500, 70000, 500):
+            a[:, :, p:p + 500] = a[:, :, :500]
+    buf = torch.zeros(c.bytes, dtype=torch.uint8, device="cuda")
+    dk, dv = dev(np.tile(k, (1, 140, 1, 1))), dev(np.tile(v, (1, 140, 1, 1)))
+    ds = dev(np.zeros(2, np.int32))
+    c.write(buf.data_ptr(), dk.data_ptr(), dv.data_ptr(), 70000, ds.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    attend(c, o, buf, dtabs, tabs, shape, rng, 1, 1, [69999, 3], None, 70000)
+
+
 @pytest.mark.parametrize("bits,dim,group,rows", [(4, 64, 1, 5), (8, 64, 2, 3), (4, 128, 4, 7), (8, 96, 3, 33), (4, 64, 1, 100),
                                                  (4, 256, 1, 20), (8, 128, 1, 40)])
 def test_many_rows(sm, dtabs, tabs, bits, dim, group, rows):
