@@ -1339,6 +1339,7 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     if (!p) return fail(SM_E_ARG, "sm_plate8_product: null plate");
     if (rows < 0 || rows > SM_PLATE8_ROWS) return fail(SM_E_ARG, "sm_plate8_product: rows out of range");
     if (!rows) return SM_OK;
+    if ((i64)rows * p->nout > ((i64)1 << 35)) return fail(SM_E_ARG, "sm_plate8_product: more than 2^35 results in one call");
     if (!X || !out || !work) return fail(SM_E_ARG, "sm_plate8_product: null argument");
     if (x_stride < p->nin || out_stride < p->nout) return fail(SM_E_ARG, "sm_plate8_product: a row stride is shorter than its row");
     if (((uintptr_t)X | (uintptr_t)out) & 7 || (uintptr_t)work & 15) return fail(SM_E_ARG, "sm_plate8_product: alignment (rows 8 bytes, work 16)");
@@ -1360,14 +1361,18 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     const int nt = (a.N + 15) / 16, rts = (rows + 15) / 16;
     if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
     else if (rts == 2) launch(g_kt.stages, "plate8.rows", k_narrow_rows<2, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
-    else if (rows <= 256) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 1>, dim3((unsigned)(nt + 3) / 4, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
     else {
+        // Tiles of 128 x 128 from 128 of them on, below that a wave a column tile (400 rows: 4096 -> 4096, 128 tiles, 32.8 us
+        // and 35.5; 768 -> 2304, 72 tiles, 18.0 and 13.7; 256 rows 1024 -> 11008, 172 tiles, 20.4 and 20.7).  Tiles of 256 x 256,
+        // one a CU, where they take fewer rounds of the GPU than those of 128, two a CU and a fifth slower: 1024 rows
+        // 1024 -> 11008, 172 of them, 36.8 us and 40.9; 2048 rows, 344, 81.8 and 69.5; 2048 rows 4096 -> 4096, 128, 76 and 58
+        const i64 t128 = (i64)((rts + 7) / 8) * ((nt + 7) / 8), t256 = (i64)((rts + 15) / 16) * ((nt + 15) / 16);
         auto tiles = [&](auto kern, int rt, int ct, int threads) {
             const int tr = (rts + rt - 1) / rt, tc = (nt + ct - 1) / ct;
-            launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)((tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
+            launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)(((i64)tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
         };
-        // (256 x 256 tiles from three quarters of a tile a CU on; they are then too large for a result that stays cached)
-        if ((i64)((rts + 15) / 16) * ((nt + 15) / 16) >= 192) tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512);
+        if (t128 < 128) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 1>, dim3((unsigned)(nt + 3) / 4, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
+        else if (8 * ((t256 + 255) / 256) <= 5 * ((t128 + 511) / 512)) tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512);
         else if ((i64)rows * a.N * 8 >= NARROW_STREAM) tiles(k_narrow_tiles<2, 2, 4, 4, true>, 8, 8, 256);
         else tiles(k_narrow_tiles<2, 2, 4, 4, false>, 8, 8, 256);
     }
@@ -1451,7 +1456,10 @@ struct NarrowWork { bool sweep; i64 q8, eq, pos, pm, pA, pE, pN, bytes; };
 static NarrowWork narrow_work(const NarrowShape& s, int R, int J) {
     const i64 n = (i64)s.streams * s.heads * R;
     NarrowWork w{};
-    w.sweep = R > 16 && (i64)s.streams * s.heads * ((R + 15) / 16) >= 256;
+    // The sweep from 640 row tiles on (one a wave's quarter), below that chunks spread over the GPU: 16 streams of 8 heads at
+    // 16,000 positions, 20 rows (256 tiles) 176 us swept and 100 split, 100 rows (896) 251 and 256; 4 streams of 32 heads over
+    // 8 at 3,000, 40 rows (320) 47 and 52, 100 rows (800) 80 and 92.  And where the chunks' sums would pass 4 GB.
+    w.sweep = R > 16 && ((i64)s.streams * s.heads * ((R + 15) / 16) >= 640 || n * J * s.wide * 4 > ((i64)4 << 30));
     w.pm = 0;
     w.pE = up256(n * J * 4);
     w.pA = w.q8 = w.pE + up256(n * J * 4);

@@ -49,7 +49,8 @@ def rows_of(rng, shape, lo=0, hi=40):
 # ---- the product
 @pytest.mark.parametrize("rows,nin,nout", [(1, 768, 2304), (1, 1, 1), (2, 63, 17), (16, 64, 16), (17, 65, 15), (31, 129, 48),
                                            (33, 1000, 33), (64, 320, 100), (65, 2051, 31), (129, 200, 70), (300, 72, 130),
-                                           (1, 9001, 5), (3, 20000, 20)])
+                                           (1, 9001, 5), (3, 20000, 20), (700, 130, 1000),
+                                           (1025, 64, 2100), (130, 100, 16500), (400, 200, 300)])
 def test_product(sm, rows, nin, nout):
     rng = np.random.default_rng(rows * 7 + nin)
     w, e, b = plate(rng, nin, nout)
@@ -279,15 +280,17 @@ def test_many_rows(sm, dtabs, tabs, bits, dim, group, rows):
     attend(c, o, buf, dtabs, tabs, shape, rng, group, rows, [400, 200, 250, -200], None, 260)
 
 
-@pytest.mark.parametrize("bits,dim,group,rows,ctx", [(4, 64, 2, 17, 700), (8, 128, 1, 40, 600), (4, 256, 3, 20, 300), (8, 64, 1, 33, 1100),
-                                                     (4, 100, 1, 36, 530), (8, 200, 2, 18, 270), (4, 40, 5, 9, 1030)])
+@pytest.mark.parametrize("bits,dim,group,rows,ctx", [(4, 64, 2, 17, 700), (8, 128, 1, 40, 600), (4, 64, 2, 50, 700), (8, 128, 1, 100, 600),
+                                                     (4, 256, 3, 40, 300), (8, 64, 1, 113, 1100), (4, 100, 1, 97, 530), (8, 200, 2, 60, 270),
+                                                     (4, 40, 5, 21, 1030), (4, 128, 2, 49, 520)])
 def test_prompt_rows(sm, dtabs, tabs, bits, dim, group, rows, ctx):
-    """enough row tiles for the sweep: prompts of uneven lengths at uneven places, some not there at all"""
+    """several and many row tiles (split over chunks, and swept): prompts of uneven lengths at uneven places, some not there
+    at all"""
     shape = (8, 12, dim, ctx, bits)
     rng = np.random.default_rng(rows)
     c, o, buf = filled_by_columns(sm, rng, shape)
     start = [ctx - rows, 0, 250, -2, 5, ctx - 3, ctx + 5, 255]
-    attend(c, o, buf, dtabs, tabs, shape, rng, group, rows, start, [rows, 2, 0, 4, -1, rows, rows, 1], ctx)
+    attend(c, o, buf, dtabs, tabs, shape, rng, group, rows, start, [min(rows, 19), 2, 0, 4, -1, rows, rows, 1], ctx)
 
 
 def filled_by_columns(sm, rng, shape):
@@ -321,7 +324,7 @@ def test_sweep_levels_far_apart(sm, dtabs, tabs):
         for name in ("k", "v", "kl", "vl"):
             getattr(wide, name)[:] = getattr(o, name)
         for scale in (None, 0, -(64 << 16), 64 << 16, 77777):
-            attend(big, wide, one.expand(96, -1).contiguous(), dtabs, tabs, shape, rng, 1, 40, [240] * 8, [2, 0, 1, 0, 0, 0, 3, 0], shape[3],
+            attend(big, wide, one.expand(96, -1).contiguous(), dtabs, tabs, shape, rng, 1, 100, [170] * 8, [2, 0, 1, 0, 0, 0, 3, 0], shape[3],
                    scale, 0, 61)
 
 
