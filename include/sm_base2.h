@@ -255,8 +255,10 @@ int64_t sm_plate_bytes(const sm_plate* p);
  * own (base2.py:18-53, 85-100) on fewer.  With rsh(x, s) = x 2^-s rounded half up, a row's digits of b bits are
  *     sh = max(bitlen(OR |x|) - (b - 1), 0),   digit = clamp(rsh(x, sh), -2^(b-1), 2^(b-1) - 1)   worth digit 2^sh.
  * Calls only launch kernels on their stream: none allocates, waits or keeps anything, so all may be captured into a graph,
- * and calls may overlap where their outputs, caches and workspaces are their own.  A call runs on the device that holds
- * the plate or the cache, whatever device is current; its stream has to be one of that device.
+ * and calls may overlap where their outputs, written caches and workspaces are their own (two graphs that may run at once
+ * have a workspace each).  Outputs overlap no input.  A call runs on the device that holds the plate or the cache, whatever
+ * device is current; its stream, its other buffers and its tables have to be that device's.  Sizes that a launch could not
+ * hold are refused with SM_E_ARG.
  * ------------------------------------------------------------------------------------------------- */
 #define SM_PLATE8_NIN 131071      /* a pile of 8-bit digits stays within int32 */
 #define SM_PLATE8_ROWS (1 << 20)
@@ -270,7 +272,7 @@ int64_t sm_plate8_work(const sm_plate8* p, int32_t rows);        /* bytes of wor
 /* out[r][j] = rsh(sum_i x8[r][i] w[i][j], -(e[j] + ex[r] + 16)) + b[j] for r < rows, with row r's 8-bit digits x8 and their
  * level ex = sh - 16: a scale for each token and each channel.  X: device int64 rows at 2^-16, x_stride values apart; out:
  * device int64 rows, out_stride apart.  work: sm_plate8_work bytes of device memory at 16 bytes' alignment, used until the
- * call's kernels have run.  rows 0 .. SM_PLATE8_ROWS. */
+ * call's kernels have run.  rows 0 .. SM_PLATE8_ROWS, at most 2^35 results a call. */
 int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x_stride, int32_t rows, int64_t* out, int64_t out_stride,
                       void* work, int64_t work_bytes, void* stream);
 
@@ -302,7 +304,8 @@ int sm_narrow_read(const sm_narrow* c, const void* cache, int64_t* k, int64_t* v
  *         A = sum u_i, N = rsh(sum_i rsh(u_i, E - level_i) v_i, 8)
  *     the row, with its chunks' largest m and E as M and L and f = ARR[M - m]
  *         out = power(sum rsh(N f, 24 + L - E), (L + 8) 65536 - log2fix(sum rsh(A f, 24)))
- * Every sum is exact, so no launch shape changes a result.  q, out: device int64, strides in values as for k.
+ * Every sum is exact, so no launch shape changes a result.  q, out: device int64, strides in values as for k.  The tables'
+ * arrival has to be base2_convert.py:50-53's (SM_E_ARG otherwise: its entries are formed as products, not gathered).
  * work: sm_narrow_work bytes of device memory at 16 bytes' alignment, used until the call's kernels have run. */
 int64_t sm_narrow_work(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span);   /* negative on error */
 int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const void* cache, const int64_t* q, int64_t q_row,

@@ -287,6 +287,7 @@ struct sm_tables {
     // e^(-d / 1024) for d < 128, where their product rounds to ARR[d] for every d up to alen (else null)
     int* ARR2 = nullptr;
     double* ARRF = nullptr;
+    int dev = -1;             // the device that holds the tables
     int alen = 0;
     i64 log768 = 0, eps40 = 0;
     int verified = 0;         // every entry equals its defining formula (checked on the device at create)
@@ -319,6 +320,7 @@ static int tables_init(sm_tables& T, const i64* phi, const i64* arr, int alen, c
                        i64 log768, i64 eps40) {
     if (alen <= 0 || alen > (1 << 20)) return fail(SM_E_ARG, "arrival table length");
     int rc;
+    HIP_TRY(hipGetDevice(&T.dev));
     if ((rc = upload_table(&T.PHI, phi, 65536, 0, 65536, "phi"))) return rc;
     if ((rc = upload_table(&T.ARR, arr, alen, 0, 1 << 24, "arrival"))) return rc;
     {

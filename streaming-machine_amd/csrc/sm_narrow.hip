@@ -1362,16 +1362,17 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     if (rts == 1) launch(g_kt.stages, "plate8.rows", k_narrow_rows<1, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
     else if (rts == 2) launch(g_kt.stages, "plate8.rows", k_narrow_rows<2, 1, 4>, dim3(nt, 1), dim3(NTHREADS), 0, s, a);
     else {
-        // Tiles of 128 x 128 from 128 of them on, below that a wave a column tile (400 rows: 4096 -> 4096, 128 tiles, 32.8 us
-        // and 35.5; 768 -> 2304, 72 tiles, 18.0 and 13.7; 256 rows 1024 -> 11008, 172 tiles, 20.4 and 20.7).  Tiles of 256 x 256,
-        // one a CU, where they take fewer rounds of the GPU than those of 128, two a CU and a fifth slower: 1024 rows
+        // Up to 64 rows a block a column tile, which then reads its weights once (64 rows 768 -> 50257 17.2 us, 21.1 in tiles of
+        // 128 x 128).  More rows in such tiles from 128 of them on (512 rows 4096 -> 4096, 128 tiles, 33.7 us against 39.8;
+        // 256 rows, 64 tiles, 31.2 against 23.7; 512 rows 1024 -> 11008, 344 tiles, 25.0 against 31.1).  Tiles of 256 x 256, one
+        // a CU, where they take fewer rounds of the GPU than those of 128, two a CU and a fifth slower: 1024 rows
         // 1024 -> 11008, 172 of them, 36.8 us and 40.9; 2048 rows, 344, 81.8 and 69.5; 2048 rows 4096 -> 4096, 128, 76 and 58
         const i64 t128 = (i64)((rts + 7) / 8) * ((nt + 7) / 8), t256 = (i64)((rts + 15) / 16) * ((nt + 15) / 16);
         auto tiles = [&](auto kern, int rt, int ct, int threads) {
             const int tr = (rts + rt - 1) / rt, tc = (nt + ct - 1) / ct;
             launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)(((i64)tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
         };
-        if (t128 < 128) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 1>, dim3((unsigned)(nt + 3) / 4, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
+        if (rows <= 64 || t128 < 128) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3((unsigned)nt, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
         else if (8 * ((t256 + 255) / 256) <= 5 * ((t128 + 511) / 512)) tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512);
         else if ((i64)rows * a.N * 8 >= NARROW_STREAM) tiles(k_narrow_tiles<2, 2, 4, 4, true>, 8, 8, 256);
         else tiles(k_narrow_tiles<2, 2, 4, 4, false>, 8, 8, 256);
@@ -1384,7 +1385,8 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
 static int narrow_shape(const sm_narrow* c, NarrowShape& s, const char* who) {
     const std::string w(who);
     if (!c) return fail(SM_E_ARG, w + ": null shape");
-    if (c->streams < 1 || c->streams > 65535 || c->heads < 1 || c->heads > 65535) return fail(SM_E_ARG, w + ": streams and heads are 1 .. 65535");
+    if (c->streams < 1 || c->streams > 65535 || c->heads < 1 || c->heads > 65535 || (i64)c->streams * c->heads > (1 << 20))
+        return fail(SM_E_ARG, w + ": streams and heads are 1 .. 65535, their product at most 2^20");
     if (c->dim < 1 || c->dim > 256) return fail(SM_E_ARG, w + ": a head has 1 .. 256 dimensions");
     if (c->ctx < 1 || c->ctx > (1 << 24)) return fail(SM_E_ARG, w + ": ctx is 1 .. 2^24");
     if (c->bits != 4 && c->bits != 8) return fail(SM_E_ARG, w + ": digits of 4 or 8 bits");
@@ -1476,7 +1478,8 @@ static int narrow_att_args(const sm_narrow* c, int32_t q_heads, int32_t rows, in
     if (q_heads < 1 || q_heads > 65535 || q_heads % s.heads) return fail(SM_E_ARG, w + ": query heads are a multiple of the cache's heads");
     if (rows < 0 || rows > s.ctx) return fail(SM_E_ARG, w + ": rows are 0 .. ctx");
     if (span < 1 || span > s.ctx) return fail(SM_E_ARG, w + ": span is 1 .. ctx");
-    if ((i64)rows * q_heads > (1 << 22)) return fail(SM_E_ARG, w + ": rows x query heads are at most 2^22");
+    if ((i64)rows * q_heads > (1 << 22) || (i64)s.streams * rows * q_heads > (1 << 26))
+        return fail(SM_E_ARG, w + ": rows x query heads are at most 2^22, over all streams 2^26");
     return SM_OK;
 }
 extern "C" int64_t sm_narrow_work(const sm_narrow* c, int32_t q_heads, int32_t rows, int32_t span) {
@@ -1541,6 +1544,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     if (!t->ARRF || t->alen > SWEEP_ARR) return fail(SM_E_ARG, "sm_narrow_attend: the tables' arrival is not base2_convert.py's");
     OnDevice on(buf);
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_attend: the cache is not in a device's memory");
+    if (on.dev != t->dev) return fail(SM_E_ARG, "sm_narrow_attend: the tables are another device's");
     char* wk = static_cast<char*>(work);
     a.buf = static_cast<const char*>(buf);
     a.q = (const i64*)q; a.q_row = q_row; a.q_stream = q_stream; a.out = (i64*)out; a.o_row = out_row; a.o_stream = out_stream;

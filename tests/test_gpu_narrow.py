@@ -355,6 +355,133 @@ def test_empty_cache_and_equal_scores(sm, dtabs, tabs):
     assert np.array_equal(out.cpu().numpy(), want)
 
 
+def test_past_four_gigabytes(sm, dtabs, tabs):
+    """the last stream's last head of a cache of 10.8 GB, at its context's end"""
+    streams, heads, dim, ctx, bits = shape = (40, 8, 256, 65536, 8)
+    rng = np.random.default_rng(4)
+    c, o = sm.NarrowCache(*shape), orc.Cache(1, 1, dim, 70, bits)
+    assert c.bytes > 2 * 2 ** 32
+    buf = torch.zeros(c.bytes, dtype=torch.uint8, device="cuda")
+    k, v = (rows_of(rng, (1, 70, 1, dim), 12, 20) for _ in range(2))
+    o.write(k, v, [0])
+    wide = torch.zeros((streams, 70, heads, dim), dtype=torch.int64, device="cuda")
+    dk, dv = wide.clone(), wide.clone()
+    dk[-1, :, -1], dv[-1, :, -1] = dev(k[0, :, 0]), dev(v[0, :, 0])
+    start, count = np.full(streams, ctx - 70, np.int32), np.zeros(streams, np.int32)
+    count[-1] = 70
+    ds, dc = dev(start), dev(count)
+    c.write(buf.data_ptr(), dk.data_ptr(), dv.data_ptr(), 70, ds.data_ptr(), dc.data_ptr(), stream=stream())
+    k2, v2 = wide.clone(), wide.clone()
+    c.read(buf.data_ptr(), k2.data_ptr(), v2.data_ptr(), 70, ds.data_ptr(), dc.data_ptr(), stream=stream())
+    wk, wv = np.zeros((1, 70, 1, dim), np.int64), np.zeros((1, 70, 1, dim), np.int64)
+    o.read(70, [0], None, wk, wv)
+    assert np.array_equal(k2[-1, :, -1].cpu().numpy(), wk[0, :, 0]) and np.array_equal(v2[-1, :, -1].cpu().numpy(), wv[0, :, 0])
+    assert int(k2[:-1].abs().sum()) == 0
+    # the same 70 rows at the front of the last stream: what a row sees there
+    start[-1] = 0
+    ds = dev(start)
+    c.write(buf.data_ptr(), dk.data_ptr(), dv.data_ptr(), 70, ds.data_ptr(), dc.data_ptr(), stream=stream())
+    q = rows_of(rng, (1, 1, 1, dim), 14, 18)
+    dq, out = torch.zeros((streams, 1, heads, dim), dtype=torch.int64, device="cuda"), torch.zeros((streams, 1, heads, dim), dtype=torch.int64, device="cuda")
+    dq[-1, 0, -1] = dev(q[0, 0, 0])
+    start[-1], count[-1] = 69, 1
+    ds, dc = dev(start), dev(count)
+    n = c.work_bytes(heads, 1, 100)
+    wk = space(n)
+    c.attend(dtabs, buf.data_ptr(), dq.data_ptr(), heads, 1, 100, ds.data_ptr(), dc.data_ptr(), out.data_ptr(), wk.data_ptr(), n, stream=stream())
+    want = np.zeros((1, 1, 1, dim), np.int64)
+    o.attend(tabs, q, [69], None, 100, c.scale, want)
+    assert np.array_equal(out[-1, 0, -1].cpu().numpy(), want[0, 0, 0])
+
+
+def test_two_streams_at_once(sm, dtabs, tabs):
+    """calls on two streams over one cache and one plate, each with its own workspace and outputs, 20 times over"""
+    rng = np.random.default_rng(2)
+    shape = (3, 2, 64, 1400, 4)
+    c, o, buf = filled_by_columns(sm, rng, shape)
+    w, e, b = plate(rng, 512, 700, True)
+    p = sm.Plate8(w, e, b)
+    X, q = rows_of(rng, (40, 512), 10, 20), rows_of(rng, (3, 2, 4, 64), 12, 18)
+    want, att = orc.product(X, w, e, b), np.zeros(q.shape, np.int64)
+    o.attend(tabs, q, [1398, 700, 3], None, 1400, c.scale, att)
+    x, dq, ds = dev(X), dev(q), dev(np.array([1398, 700, 3], np.int32))
+    pn, an = p.work_bytes(40), c.work_bytes(4, 2, 1400)
+    torch.cuda.synchronize()
+    sides = []
+    for _ in range(2):
+        st = torch.cuda.Stream()
+        sides.append((st, torch.zeros((40, 700), dtype=torch.int64, device="cuda"), torch.zeros(q.shape, dtype=torch.int64, device="cuda"),
+                      space(pn), space(an)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, out, ao, pw, aw in sides:
+            p.product(x.data_ptr(), 40, out.data_ptr(), pw.data_ptr(), pn, stream=st.cuda_stream)
+            c.attend(dtabs, buf.data_ptr(), dq.data_ptr(), 4, 2, 1400, ds.data_ptr(), 0, ao.data_ptr(), aw.data_ptr(), an, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for _, out, ao, _, _ in sides:
+        assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(ao.cpu().numpy(), att)
+
+
+def test_graph_of_a_prompt(sm, dtabs, tabs):
+    """write and swept attention captured once, replayed on new rows with eager calls and waits between"""
+    rng = np.random.default_rng(9)
+    shape = (8, 12, 64, 300, 4)
+    c, o = sm.NarrowCache(*shape), orc.Cache(*shape)
+    buf = torch.zeros(c.bytes, dtype=torch.uint8, device="cuda")
+    rows = 100
+    k, v, q, out = (torch.zeros((8, rows, 12, 64), dtype=torch.int64, device="cuda") for _ in range(4))
+    ds, dc = torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    n = c.work_bytes(12, rows, 300)
+    wk = space(n)
+
+    def calls():
+        c.write(buf.data_ptr(), k.data_ptr(), v.data_ptr(), rows, ds.data_ptr(), dc.data_ptr(), stream=stream())
+        c.attend(dtabs, buf.data_ptr(), q.data_ptr(), 12, rows, 300, ds.data_ptr(), dc.data_ptr(), out.data_ptr(), wk.data_ptr(), n, stream=stream())
+
+    calls()                                         # (nothing there: count 0)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        calls()
+    for i in range(3):
+        new = [rows_of(rng, (1, rows, 1, 64), 12, 18).repeat(8, 0).repeat(12, 2) for _ in range(3)]
+        start, count = np.full(8, 100 * i, np.int32), np.array([3, 0, 1, 0, 0, 2, 0, 0], np.int32) if i else np.full(8, rows, np.int32)
+        for t, a in zip((k, v, q), new):
+            t.copy_(dev(a))
+        ds.copy_(dev(start))
+        if i == 0:                                  # fill every stream eagerly, then replay over it with few rows
+            dc.copy_(dev(count))
+            calls()
+            one = orc.Cache(1, 1, 64, 300, 4)
+            one.write(new[0][:1, :, :1], new[1][:1, :, :1], [0])
+            for name in ("k", "v", "kl", "vl"):
+                getattr(o, name)[:, :, :rows] = getattr(one, name)[:, :, :rows]
+            count = np.array([0, 2, 0, 0, 1, 0, 0, 0], np.int32)
+        dc.copy_(dev(count))
+        out.fill_(55)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        o.write(new[0], new[1], start, count)
+        want = np.full(tuple(out.shape), 55, np.int64)
+        o.attend(tabs, new[2], start, count, 300, c.scale, want)
+        assert np.array_equal(out.cpu().numpy(), want), i
+        calls()
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want), i
+
+
+def test_other_tables_are_refused(sm, tabs):
+    """an arrival that is not base2_convert.py's (its products would not be it)"""
+    t = sm.Tables({**tabs, "arrival": tabs["arrival"][:-5]})
+    c = sm.NarrowCache(1, 1, 64, 64, 4)
+    buf, x = torch.zeros(c.bytes, dtype=torch.uint8, device="cuda"), torch.zeros(64, dtype=torch.int64, device="cuda")
+    wk, ds = space(c.work_bytes(1, 1, 64)), dev(np.zeros(1, np.int32))
+    with pytest.raises(sm.SmError) as e:
+        c.attend(t, buf.data_ptr(), x.data_ptr(), 1, 1, 64, ds.data_ptr(), 0, x.data_ptr(), wk.data_ptr(), wk.numel())
+    assert e.value.code == -1
+
+
 def test_host_memory_is_refused(sm, dtabs):
     c = sm.NarrowCache(1, 1, 64, 64, 4)
     a = np.zeros(c.bytes + 64, np.uint8)

@@ -133,3 +133,15 @@ def test_plates_refused(sm):
     assert L.sm_plate8_work(None, 1) == -1
     assert L.sm_plate8_create(None, None, None, 4, 3, None) == -1
     assert L.sm_plate8_destroy(None) == 0 and L.sm_plate8_bytes(None) == 0
+
+
+def test_sizes_that_no_launch_holds_are_refused(sm):
+    for shape in ((65535, 17, 64, 8, 4), (1, 70000, 64, 8, 4)):
+        with pytest.raises(sm.SmError) as e:
+            sm.NarrowCache(*shape)
+        assert e.value.code == -1
+    c = sm.NarrowCache(64, 64, 128, 1 << 20, 4)
+    assert c.bytes == 64 * 64 * (1 << 14) * (16 * 128 * 4 + 128)
+    refused(sm, lambda: c.work_bytes(64, (1 << 16) + 1, 1 << 20))
+    refused(sm, lambda: c.work_bytes(64, (1 << 14) + 1, 1 << 20))
+    assert 0 < c.work_bytes(64, 1, 1 << 20) < 1 << 40
