@@ -87,8 +87,9 @@ SMD i64x2 row_pair(const i64* x, int i, int nin) {
 // One block a row: the row's level, then its digits in the operand's order.  A thread loads two values in a row, so that a
 // wave's load is 1 KB in a row (16 bytes every 32, four values a thread, touch each line twice: 53 us at 4096 rows of 4096),
 // and pairs of threads swap halves to store four digits each.  Rows of up to 8,192 values are held in registers between the
-// two passes, longer ones are read again.  Bound by the rows' read.  The 16 rows of a tile share their 128-byte lines of
-// digits: with many rows, blocks of one die (every eighth) take one tile, so that the lines fill in that die's L2.
+// two passes, longer ones are read again.  The 16 rows of a tile share their 128-byte lines of digits: with many rows,
+// blocks of one die (every eighth) take one tile, so that the lines fill in that die's L2.  Bound by the rows' read: 4096
+// rows of 4096 in 31 us, 4.9 TB/s.
 __global__ __launch_bounds__(NTHREADS) void k_narrow_lights(Narrow8Args a) {
     constexpr int HOLD = 8, STEP = 4 * NTHREADS;
     __shared__ u64 wor[NTHREADS / 64];
@@ -201,7 +202,9 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_one(Narrow8Args a) {
     a.out[(i64)row * a.ldo + col] = narrow_out(pile, a.we[col], lev[row], a.wb[col]);
 }
 
-// RT row tiles by CT column tiles a wave, the inputs split over KW of a block's four waves and their piles added
+// RT row tiles by CT column tiles a wave, the inputs split over KW of a block's four waves and their piles added: weights and
+// lights straight from memory into operands, four steps' loads in flight.  Bound by the weights' read and the results' write:
+// 64 rows 768 -> 50257 in 17.5 us, 3.7 TB/s; a column tile a wave without the split took 52 us against 25 at 8192 -> 8192.
 template <int RT, int CT, int KW>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
     constexpr int CG = 4 / KW, TILES = RT * CT;
@@ -258,7 +261,9 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_rows(Narrow8Args a) {
 
 // The product of many rows: WR x WC waves of RT x CT tiles each.  Every step of 64 inputs is a stage of (WR RT + WC CT)
 // fragments of 1 KB, loaded from memory straight into LDS in the operands' order (so neither the loads nor the operand
-// reads rearrange anything and no two lanes meet in a bank), ST - 1 stages ahead.
+// reads rearrange anything and no two lanes meet in a bank), three stages ahead; a stage's operands are read into registers
+// while the stage before is multiplied (255 us at 4096 rows 4096 -> 11008 with the reads in the same step, 200 so).  Bound by
+// the matrix units: 1,850 TOP/s there with the results' 360 MB written (a large library product of bytes reaches 2,285).
 typedef const __attribute__((address_space(1))) void* gas_p;
 typedef __attribute__((address_space(3))) void* las_p;
 template <int WR, int WC, int RT, int CT, bool NT>
@@ -400,10 +405,11 @@ SMD void narrow_range(const int* start, const int* count, int stream, int rows, 
 
 // A block a (tile, head, stream): its rows' levels and digits (a wave a row, four rows' loads in flight), through LDS in the
 // units' order (a dimension's positions 16 t + 4 g + r at byte 16 g + 4 t + r), then whole 16-byte units; a unit of values is
-// read first where it also holds positions that the call does not write.  Bound by the rows' read.
-template <int BITS, int WIDE>
-__global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
-    constexpr int PER = WIDE / 64, AT_ONCE = PER == 4 ? 2 : 4, NW = NTHREADS / 64;
+// read first where it also holds positions that the call does not write.  Bound by the rows' read: three prompts of 2,048
+// rows of 8 heads of 128 in 19 us, 4.5 TB/s.
+template <int BITS, int WIDE, int NW>
+__global__ __launch_bounds__(64 * NW) void k_narrow_write(NarrowRows a) {
+    constexpr int PER = WIDE / 64, AT_ONCE = PER == 4 ? 2 : 4;
     __shared__ __attribute__((aligned(16))) signed char kd[64][WIDE + 4], vd[WIDE][68];
     // (the heads first: blocks that run together read whole rows)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x % a.s.heads, stream = blockIdx.z;
@@ -454,7 +460,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
     auto halves = [](int x, int y) { return (int)(((unsigned)x & 0x0F0F0F0Fu) | ((unsigned)y & 0x0F0F0F0Fu) << 4); };
     constexpr int UNITS = WIDE * BITS / 128;                     // 16-byte units a position, or a dimension's 64 / 4
     const bool whole = b0 == 0 && b1 == 63;
-    for (int i = tid; i < UNITS * 64; i += NTHREADS) {
+    for (int i = tid; i < UNITS * 64; i += 64 * NW) {
         const int c = i >> 6, b = i & 63;
         if (b < b0 || b > b1) continue;
         const int* row = reinterpret_cast<const int*>(kd[b]);
@@ -464,7 +470,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
         *reinterpret_cast<v4i*>(base + (i64)i * 16) = w;
     }
     char* vbase = base + narrow_half(a.s);
-    for (int i = tid; i < UNITS * 64; i += NTHREADS) {
+    for (int i = tid; i < UNITS * 64; i += 64 * NW) {
         const int c = i >> 6, g = (i >> 4) & 3, m = i & 15;
         v4i w;
 #pragma unroll
@@ -498,7 +504,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_write(NarrowRows a) {
 }
 
 // A thread two dimensions of a (row, head), k and v: 16-byte stores (rows stand at 8 bytes' alignment only).  Bound by what it
-// writes, eight bytes or more a digit.
+// writes, eight bytes a digit: the same three prompts in 16 us, 5.1 TB/s.
 template <int BITS, bool NT>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_read(NarrowRows a) {
     const int stream = blockIdx.z, pairs = (a.s.dim + 1) / 2, hd = a.s.heads * pairs;
@@ -738,7 +744,9 @@ SMD double narrow_joined(double N, int Nj, double f) { return N + floor(__builti
 // Few rows: a wave a chunk, a tile of GR rows (RU of every four wanted).  Scores: A = q, B = keys, so a lane is a position.
 // With fewer than 16 rows the rows of position tile t' stand in operand rows GR t' .., zeros elsewhere, and 16 / GR position
 // tiles add into one accumulator: every lane then holds a score that is wanted.  Weights: byte planes through the wave's
-// LDS, their planes stacked as rows of one operand (3 GR rows in NM operands).
+// LDS, their planes stacked as rows of one operand (3 GR rows in NM operands).  All of a chunk's keys are asked for first, then
+// its values (in the registers that AHEAD tiles take).  Bound by the cache's read: 64 streams of up to 8,192 positions, 4 rows
+// a key head, 4 bits, in 73 us, 4.7 TB/s; 131,072 positions of 8 bits in 63 us, 4.3 TB/s.
 template <int BITS, int DK, int GR, int RU> struct NarrowChunk {
     static constexpr int NA = GR / 4, PT = 16 / GR, NM = (3 * GR + 15) / 16, DT = 4 * DK, VU = 8 / BITS, WBUF = NM * 1024;
     static constexpr int TILE_DW = DK * BITS * 2;                   // registers of a tile's keys (of its values)
@@ -1001,7 +1009,9 @@ __global__ __launch_bounds__(64 * NW, DK <= 2 ? 2 : 1) void k_narrow_near(Narrow
 // B = q, so that a lane holds one row's scores of 16 positions a tile, and exactly the ones, in the order, that its bytes of a
 // weight operand are (the values' layout): nothing moves between lanes.  A first pass over the keys finds each chunk's m_j
 // and E_j (kept in memory) and the row's M and E; the second adds each chunk's N_j f_j in registers, and the waves' sums are
-// added at the end.  Bound by the vector arithmetic of a score.
+// added at the end.  Bound by the vector arithmetic of a score, 23 steps in the second pass and 5 in the first (the matrix
+// products take a fifth of that), at three waves a SIMD: 1,024 rows of two prompts over 4,096 positions, 12 heads of 64, in
+// 105 us.  (The weights from the 71 KB table in LDS: two waves, 138 us; sums in registers: 111 us.)
 #define SWEEP_WAVES 4
 template <int BITS, int DK>
 __global__ __launch_bounds__(64 * SWEEP_WAVES, 4 - (DK == 4 ? 3 : DK)) void k_narrow_sweep(NarrowAtt a) {
@@ -1427,9 +1437,15 @@ extern "C" int sm_narrow_write(const sm_narrow* c, void* buf, const int64_t* k, 
     const i64 blocks = (i64)((rows + 62) / 64 + 1) * a.s.heads;
     if (blocks > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_write: too many rows for one call");
     const dim3 grid((unsigned)blocks, 1, (unsigned)a.s.streams);
-    auto go = [&](auto kern) { launch(g_kt.stages, "narrow.write", kern, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a); };
-    if (a.s.bits == 4) a.s.wide == 64 ? go(k_narrow_write<4, 64>) : a.s.wide == 128 ? go(k_narrow_write<4, 128>) : go(k_narrow_write<4, 256>);
-    else a.s.wide == 64 ? go(k_narrow_write<8, 64>) : a.s.wide == 128 ? go(k_narrow_write<8, 128>) : go(k_narrow_write<8, 256>);
+    auto write = [&](auto nw) {
+        constexpr int NW = decltype(nw)::value;
+        auto go = [&](auto kern) { launch(g_kt.stages, "narrow.write", kern, grid, dim3(64 * NW), 0, (hipStream_t)stream, a); };
+        if (a.s.bits == 4) a.s.wide == 64 ? go(k_narrow_write<4, 64, NW>) : a.s.wide == 128 ? go(k_narrow_write<4, 128, NW>) : go(k_narrow_write<4, 256, NW>);
+        else a.s.wide == 64 ? go(k_narrow_write<8, 64, NW>) : a.s.wide == 128 ? go(k_narrow_write<8, 128, NW>) : go(k_narrow_write<8, 256, NW>);
+    };
+    // eight waves a block where a tile has rows for them (997 rows of 7 heads of 80, five streams: 14.3 us, 16.9 with four)
+    if (rows <= 8) write(std::integral_constant<int, 4>());
+    else write(std::integral_constant<int, 8>());
     HIP_TRY(hipGetLastError());
     return SM_OK;
 }
