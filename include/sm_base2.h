@@ -289,7 +289,8 @@ int64_t sm_narrow_bytes(const sm_narrow* c);                     /* negative on 
  * head)'s tile of 64 positions have to be in order. */
 int sm_narrow_write(const sm_narrow* c, void* cache, const int64_t* k, const int64_t* v, int64_t row_stride,
                     int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream);
-/* The same rows back: what the digits stand for, digit 2^sh.  Rows that are left out stay as they are in k and v. */
+/* The same rows back: what the digits stand for, digit 2^sh.  Rows that are left out stay as they are in k and v.  Strides
+ * that lay rows over one another are refused. */
 int sm_narrow_read(const sm_narrow* c, const void* cache, int64_t* k, int64_t* v, int64_t row_stride,
                    int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream);
 /* Attention of `rows` rows a stream over the cache: row t < count[s] of stream s is at position p = start[s] + t, and each of

@@ -1425,6 +1425,11 @@ static int narrow_rows(const sm_narrow* c, const void* buf, const void* k, const
     return SM_OK;
 }
 
+// whether rows of `width` values of several streams would lie over one another (results may not)
+static bool rows_overlap(int streams, int rows, i64 width, i64 row, i64 stream) {
+    return streams > 1 && stream < (rows - 1) * row + width && (stream < width || (rows > 1 && row < (streams - 1) * stream + width));
+}
+
 extern "C" int sm_narrow_write(const sm_narrow* c, void* buf, const int64_t* k, const int64_t* v, int64_t row_stride,
                                int64_t stream_stride, int32_t rows, const int32_t* start, const int32_t* count, void* stream) {
     NarrowRows a{};
@@ -1435,7 +1440,7 @@ extern "C" int sm_narrow_write(const sm_narrow* c, void* buf, const int64_t* k, 
     a.buf = static_cast<char*>(buf); a.k = (const i64*)k; a.v = (const i64*)v;
     a.row_stride = row_stride; a.stream_stride = stream_stride; a.rows = rows; a.start = start; a.count = count;
     const i64 blocks = (i64)((rows + 62) / 64 + 1) * a.s.heads;
-    if (blocks > (1 << 23)) return fail(SM_E_ARG, "sm_narrow_write: too many rows for one call");
+    if (blocks > (1 << 22)) return fail(SM_E_ARG, "sm_narrow_write: too many rows for one call");
     const dim3 grid((unsigned)blocks, 1, (unsigned)a.s.streams);
     auto write = [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
@@ -1455,6 +1460,7 @@ extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, i
     NarrowRows a{};
     int rc = narrow_rows(c, buf, k, v, row_stride, stream_stride, rows, start, a.s, "sm_narrow_read");
     if (rc || !rows) return rc;
+    if (rows_overlap(a.s.streams, rows, (i64)a.s.heads * a.s.dim, row_stride, stream_stride)) return fail(SM_E_ARG, "sm_narrow_read: the strides lay rows over one another");
     OnDevice on(buf);
     if (!on.ok) return fail(SM_E_ARG, "sm_narrow_read: the cache is not in a device's memory");
     a.buf = static_cast<char*>(const_cast<void*>(buf)); a.k2 = (i64*)k; a.v2 = (i64*)v;
@@ -1550,6 +1556,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     if (!buf || !q || !start || !out || !work) return fail(SM_E_ARG, "sm_narrow_attend: null argument");
     const i64 width = (i64)q_heads * a.s.dim;
     if (q_row < width || out_row < width || q_stream < 0 || out_stream < 0) return fail(SM_E_ARG, "sm_narrow_attend: strides");
+    if (rows_overlap(a.s.streams, rows, width, out_row, out_stream)) return fail(SM_E_ARG, "sm_narrow_attend: the strides lay results over one another");
     if (scale < -(64 << 16) || scale > (64 << 16)) return fail(SM_E_ARG, "sm_narrow_attend: the scale's log2 is out of range");
     if (((uintptr_t)buf | (uintptr_t)work) & 15 || ((uintptr_t)q | (uintptr_t)out) & 7 || (uintptr_t)start & 3)
         return fail(SM_E_ARG, "sm_narrow_attend: alignment (cache and work 16 bytes, rows 8)");

@@ -145,3 +145,19 @@ def test_sizes_that_no_launch_holds_are_refused(sm):
     refused(sm, lambda: c.work_bytes(64, (1 << 16) + 1, 1 << 20))
     refused(sm, lambda: c.work_bytes(64, (1 << 14) + 1, 1 << 20))
     assert 0 < c.work_bytes(64, 1, 1 << 20) < 1 << 40
+
+
+def test_results_over_one_another_are_refused(sm):
+    """outputs whose strides lay streams' rows over one another; streams between the rows of others are fine to ask for"""
+    c = sm.NarrowCache(3, 2, 64, 100, 4)
+    t = type("T", (), {"h": ctypes.c_void_p(DEV)})()
+    L = sm.lib()
+    for rows, row, stream in ((1, 128, 127), (2, 128, 128), (2, 128, 255), (4, 300, 128), (2, 383, 128)):
+        refused(sm, lambda: c.read(DEV, DEV, DEV, rows, DEV, row_stride=row, stream_stride=stream))
+        refused(sm, lambda: c.attend(t, DEV, DEV, 2, rows, 100, DEV, 0, DEV, DEV, 1 << 30, out_row=row, out_stream=stream))
+    assert L.sm_narrow_read(c._ref, DEV, DEV, DEV, 128, 0, 1, DEV, None, None) == -1
+    # dense, streams apart, and rows of all streams in turn: refused later, since the address is no device's
+    for rows, row, stream in ((2, 128, 256), (1, 128, 128), (2, 384, 128)):
+        with pytest.raises(sm.SmError) as e:
+            c.read(DEV, DEV, DEV, rows, DEV, row_stride=row, stream_stride=stream)
+        assert "device's memory" in str(e.value)
