@@ -12,7 +12,8 @@
 // Results of NARROW_STREAM bytes and more are stored past the caches (nontemporal): left in the 256 MB behind them, a large
 // result is written out while the next kernel reads, which then takes half as long again (three prompts of 2,048 rows
 // written and read back 37 against 50 us, 4,096 rows 4,096 -> 11,008 249 against 270 us).  Smaller ones stay cached for
-// whoever reads them (64 rows 768 -> 50,257 18.2 us stored past the caches, 17.2 not).
+// whoever reads them (64 rows 768 -> 50,257 18.2 us stored past the caches, 17.2 not), and so do rows that share their lines
+// of 128 bytes: past the caches such a line is written in parts (193 rows 364 -> 46,797 65 us, 33 cached).
 #define NARROW_STREAM (64 << 20)
 typedef i64 i64x2 __attribute__((ext_vector_type(2), aligned(8)));       // (rows stand at 8 bytes' alignment only)
 template <bool NT> SMD void put(i64* p, i64 v) {
@@ -1269,6 +1270,9 @@ __global__ __launch_bounds__(NTHREADS, 8) void k_narrow_join(NarrowAtt a, int db
 // ---------------------------------------------------------------------------------------------------------
 // entry points
 
+// rows of int64 that begin at lines of 128 bytes
+static bool whole_lines(const void* p, i64 stride) { return !((uintptr_t)p & 127) && stride % 16 == 0; }
+
 // The device that holds a call's memory, made current for the call.  Memory that no device holds is refused here, before a
 // kernel reads it.
 struct OnDevice {
@@ -1362,7 +1366,10 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
     a.lights = static_cast<signed char*>(work);
     a.level = reinterpret_cast<int*>(static_cast<char*>(work) + plate8_lights(p, rows));
     hipStream_t s = (hipStream_t)stream;
-    if ((i64)rows * ((p->K + 1023) / 1024) <= FEW_QUADS) {
+    // (every block forms the rows' digits: 8 rows 143 -> 36336, 2,271 blocks, 19.3 us so and 10.4 in two launches; one row
+    // 2761 -> 41192, 2,575 blocks of three, 21 us)
+    const i64 quads = (i64)rows * ((p->K + 1023) / 1024);
+    if (quads <= FEW_QUADS && quads * ((a.N + 15) / 16) <= 8192) {
         launch(g_kt.stages, "plate8.one", k_narrow_one, dim3((unsigned)((a.N + 15) / 16)), dim3(NTHREADS), 0, s, a);
         HIP_TRY(hipGetLastError());
         return SM_OK;
@@ -1377,15 +1384,15 @@ extern "C" int sm_plate8_product(const sm_plate8* p, const int64_t* X, int64_t x
         // 256 rows, 64 tiles, 31.2 against 23.7; 512 rows 1024 -> 11008, 344 tiles, 25.0 against 31.1).  Tiles of 256 x 256, one
         // a CU, where they take fewer rounds of the GPU than those of 128, two a CU and a fifth slower: 1024 rows
         // 1024 -> 11008, 172 of them, 36.8 us and 40.9; 2048 rows, 344, 81.8 and 69.5; 2048 rows 4096 -> 4096, 128, 76 and 58
+        const bool past = (i64)rows * a.N * 8 >= NARROW_STREAM && whole_lines(out, out_stride);
         const i64 t128 = (i64)((rts + 7) / 8) * ((nt + 7) / 8), t256 = (i64)((rts + 15) / 16) * ((nt + 15) / 16);
         auto tiles = [&](auto kern, int rt, int ct, int threads) {
             const int tr = (rts + rt - 1) / rt, tc = (nt + ct - 1) / ct;
             launch(g_kt.stages, "plate8.tiles", kern, dim3((unsigned)(((i64)tr * tc + 7) / 8 * 8)), dim3(threads), 0, s, a, tr, tc);
         };
         if (rows <= 64 || t128 < 128) launch(g_kt.stages, "plate8.rows", k_narrow_rows<4, 1, 4>, dim3((unsigned)nt, (unsigned)((rts + 3) / 4)), dim3(NTHREADS), 0, s, a);
-        else if (8 * ((t256 + 255) / 256) <= 5 * ((t128 + 511) / 512)) tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512);
-        else if ((i64)rows * a.N * 8 >= NARROW_STREAM) tiles(k_narrow_tiles<2, 2, 4, 4, true>, 8, 8, 256);
-        else tiles(k_narrow_tiles<2, 2, 4, 4, false>, 8, 8, 256);
+        else if (8 * ((t256 + 255) / 256) <= 5 * ((t128 + 511) / 512)) past ? tiles(k_narrow_tiles<2, 4, 8, 4, true>, 16, 16, 512) : tiles(k_narrow_tiles<2, 4, 8, 4, false>, 16, 16, 512);
+        else past ? tiles(k_narrow_tiles<2, 2, 4, 4, true>, 8, 8, 256) : tiles(k_narrow_tiles<2, 2, 4, 4, false>, 8, 8, 256);
     }
     HIP_TRY(hipGetLastError());
     return SM_OK;
@@ -1468,7 +1475,8 @@ extern "C" int sm_narrow_read(const sm_narrow* c, const void* buf, int64_t* k, i
     const i64 n = (i64)rows * a.s.heads * ((a.s.dim + 1) / 2);
     const dim3 grid((unsigned)std::min<i64>((n + NTHREADS - 1) / NTHREADS, 4096), 1, (unsigned)a.s.streams);
     auto go = [&](auto kern) { launch(g_kt.stages, "narrow.read", kern, grid, dim3(NTHREADS), 0, (hipStream_t)stream, a); };
-    const bool nt = (i64)a.s.streams * rows * a.s.heads * a.s.dim * 16 >= NARROW_STREAM;
+    const bool nt = (i64)a.s.streams * rows * a.s.heads * a.s.dim * 16 >= NARROW_STREAM && whole_lines(k, row_stride) &&
+                    whole_lines(v, row_stride) && stream_stride % 16 == 0;
     if (a.s.bits == 4) nt ? go(k_narrow_read<4, true>) : go(k_narrow_read<4, false>);
     else nt ? go(k_narrow_read<8, true>) : go(k_narrow_read<8, false>);
     HIP_TRY(hipGetLastError());
@@ -1483,7 +1491,9 @@ static NarrowWork narrow_work(const NarrowShape& s, int R, int J) {
     // The sweep from 640 row tiles on (one a wave's quarter), below that chunks spread over the GPU: 16 streams of 8 heads at
     // 16,000 positions, 20 rows (256 tiles) 176 us swept and 100 split, 100 rows (896) 251 and 256; 4 streams of 32 heads over
     // 8 at 3,000, 40 rows (320) 47 and 52, 100 rows (800) 80 and 92.  And where the chunks' sums would pass 4 GB.
-    w.sweep = R > 16 && ((i64)s.streams * s.heads * ((R + 15) / 16) >= 640 || n * J * s.wide * 4 > ((i64)4 << 30));
+    // With heads past 128 dimensions, whose chunks leave a wave a SIMD, from 256 tiles on: 2 streams of 8 heads of 256 at 1,000,
+    // 300 rows (304) 54 and 80; 200 rows of one at 6,000 (104) 106 and 72.
+    w.sweep = R > 16 && ((i64)s.streams * s.heads * ((R + 15) / 16) >= (s.wide == 256 ? 256 : 640) || n * J * s.wide * 4 > ((i64)4 << 30));
     w.pm = 0;
     w.pE = up256(n * J * 4);
     w.pA = w.q8 = w.pE + up256(n * J * 4);

@@ -63,6 +63,24 @@ def test_product(sm, rows, nin, nout):
     assert np.array_equal(out.cpu().numpy(), orc.product(X, w, e, b))
 
 
+@pytest.mark.parametrize("rows,nin,nout", [(193, 64, 46797), (260, 70, 46848), (1040, 40, 8192), (1100, 200, 16000), (8, 143, 20000)])
+def test_product_of_many_tiles(sm, rows, nin, nout):
+    """results too many for the row by row oracle: its formula over the whole array (piles below 2^53, so exact in float64)"""
+    rng = np.random.default_rng(rows)
+    w, e, b = plate(rng, nin, nout, True)
+    X = rows_of(rng, (rows, nin), 8, 24)
+    p = sm.Plate8(w, e, b)
+    x, n = dev(X), p.work_bytes(rows)
+    out, wk = torch.full((rows, nout), -7, dtype=torch.int64, device="cuda"), space(n)
+    p.product(x.data_ptr(), rows, out.data_ptr(), wk.data_ptr(), n, stream=stream())
+    x8, sh = zip(*(orc.digits(r, 8) for r in X))
+    pile = np.rint(np.array(x8, np.float64) @ w.astype(np.float64)).astype(np.int64)
+    s = -(e.astype(np.int64)[None, :] + np.array(sh, np.int64)[:, None])
+    up = np.maximum(s, 0)
+    want = np.where(s > 0, (pile + (np.int64(1) << np.maximum(s - 1, 0))) >> up, pile << np.maximum(-s, 0)) + b
+    assert np.array_equal(out.cpu().numpy(), want)
+
+
 def test_product_edges(sm):
     """rows of zeros, of the largest and smallest values, a pile at the edge of 32 bits, powers that shift everything out or
     past 64 bits, biases that wrap"""
