@@ -283,9 +283,8 @@ static void free_mfma_plate(MfmaPlate& P) {
 struct sm_tables {
     int* LOG2 = nullptr; int* EXP2 = nullptr; int* PHI = nullptr; int* ARR = nullptr;
     int* GPOW = nullptr; int* HPOW = nullptr; int* PGPOW = nullptr;
-    // the narrow attention's: [alen + 1] 2 rsh(ARR[d], 2), a 0 at the end; e^(-d / 8) 2^24 for d <= alen / 128, then
-    // e^(-d / 1024) for d < 128, where their product rounds to ARR[d] for every d up to alen (else null)
-    int* ARR2 = nullptr;
+    // the narrow attention's: e^(-d / 8) 2^24 for d <= alen / 128, then e^(-d / 1024) for d < 128, where their product rounds
+    // to ARR[d] for every d up to alen (else null)
     double* ARRF = nullptr;
     int dev = -1;             // the device that holds the tables
     int alen = 0;
@@ -324,9 +323,6 @@ static int tables_init(sm_tables& T, const i64* phi, const i64* arr, int alen, c
     if ((rc = upload_table(&T.PHI, phi, 65536, 0, 65536, "phi"))) return rc;
     if ((rc = upload_table(&T.ARR, arr, alen, 0, 1 << 24, "arrival"))) return rc;
     {
-        std::vector<i64> w(alen + 1, 0);
-        for (int d = 0; d < alen; d++) w[d] = (arr[d] + 2) >> 2 << 1;
-        if ((rc = upload_table(&T.ARR2, w.data(), w.size(), 0, 1 << 23, "arrival weights"))) return rc;
         std::vector<double> f(alen / 128 + 1 + 128);
         for (int d = 0; d <= alen / 128; d++) f[d] = std::exp(-d / 8.0) * 16777216.0;
         for (int d = 0; d < 128; d++) f[alen / 128 + 1 + d] = std::exp(-d / 1024.0);
@@ -382,7 +378,7 @@ static int stage_init(sm_tables& T) {
 }
 
 static void tables_free(sm_tables& T) {
-    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.ARR2); hfree(T.ARRF); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
+    hfree(T.LOG2); hfree(T.EXP2); hfree(T.PHI); hfree(T.ARR); hfree(T.ARRF); hfree(T.GPOW); hfree(T.HPOW); hfree(T.PGPOW); hfree(T.scratch);
     hfree(T.asc); hfree(T.acm); hfree(T.aacc); hfree(T.posn);
     if (T.herr) (void)hipHostFree(T.herr);
 }

@@ -567,7 +567,6 @@ struct NarrowAtt {
     signed char* q8;             // [streams][heads][R][wide]
     int* eq; int* pos;           // [streams][heads][R] the digits' level; the row's position, -1 a row that is not there
     int* pm; int* pA; int* pE; int* pN;     // [streams][heads][J][R] each chunk's m_j, A_j, E_j and (x wide) N_j
-    const int* W2;               // the arrivals' weights 2 rsh(ARR[d], 2), 0 at alen
     const double* WF;            // ARR's factors (sm_tables): [alen / 128 + 1], [128]
     Tables tb;
 };
@@ -1583,7 +1582,7 @@ extern "C" int sm_narrow_attend(const sm_tables* t, const sm_narrow* c, const vo
     a.q = (const i64*)q; a.q_row = q_row; a.q_stream = q_stream; a.out = (i64*)out; a.o_row = out_row; a.o_stream = out_stream;
     a.start = start; a.count = count; a.span = span; a.F = scale; a.tb = t->tb();
     a.q8 = reinterpret_cast<signed char*>(wk + w.q8); a.eq = reinterpret_cast<int*>(wk + w.eq); a.pos = reinterpret_cast<int*>(wk + w.pos);
-    a.pm = reinterpret_cast<int*>(wk + w.pm); a.W2 = t->ARR2; a.WF = t->ARRF; a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
+    a.pm = reinterpret_cast<int*>(wk + w.pm); a.WF = t->ARRF; a.pA = reinterpret_cast<int*>(wk + w.pA); a.pE = reinterpret_cast<int*>(wk + w.pE);
     a.pN = reinterpret_cast<int*>(wk + w.pN);
     hipStream_t st = (hipStream_t)stream;
     if (a.s.bits == 4) a.s.wide == 64 ? narrow_attend<4, 1>(a, w.sweep, st) : a.s.wide == 128 ? narrow_attend<4, 2>(a, w.sweep, st) : narrow_attend<4, 4>(a, w.sweep, st);
